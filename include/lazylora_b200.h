@@ -362,6 +362,81 @@ int ll_profile_launch_events(void* const* events, int n);
 int ll_profile_launch_recorded(void);
 const char* ll_profile_launch_name(int i);
 
+/* ------------------------------------------------------------------ latent attention
+ * Attention whose keys and values come from one shared latent vector per token (d_c values) and
+ * one rotary key per token (d_r values, shared by the heads). dtype: 1 = bf16, 2 = fp16 for every
+ * 16-bit tensor of a call. Strides are in elements, the innermost dimension is contiguous, every
+ * pointer is 16-byte aligned and every stride a multiple of 8. Bad device-side values (a position
+ * outside the table, a slot outside the cache, a page outside it) are skipped and recorded; a
+ * bounded wait that runs out likewise: ll_latent_status(stream) synchronises, returns the first
+ * one recorded since the last call on the current device and clears it. */
+int ll_latent_status(void* stream);
+
+/* New tokens into the paged cache [pages][page_size][d_c + d_r]: token t's row kv[t] (d_c latent
+ * values, then its d_r rotary values, not yet rotated) goes to slot slots[t] = page * page_size +
+ * offset with its rotary part turned by the angle of positions[t]; a negative slot writes nothing.
+ * table [table_rows][d_r] fp32: d_r / 2 cosines, then d_r / 2 sines. interleaved 1: pairs
+ * (2i, 2i + 1); 0: (i, i + d_r / 2). The queries' rotary parts q_pe [T][H][d_r] are turned into
+ * q_out in the same launch (H = 0, or NULL: none; q_out may be q_pe). Distinct slots. */
+int ll_latent_append(const void* kv, int64_t kv_stride, const int64_t* slots, const int64_t* positions,
+                     const float* table, int table_rows, int T, int d_c, int d_r, int dtype, int interleaved,
+                     void* cache, int64_t page_stride, int64_t row_stride, int pages, int page_size, const void* q_pe,
+                     int64_t q_stride_t, int64_t q_stride_h, int H, void* q_out, int64_t qo_stride_t,
+                     int64_t qo_stride_h, void* stream);
+
+/* The same rotation of x [T][H][d_r] into out (may be x); inverse 1 turns back (the gradient). */
+int ll_latent_rotate(const void* x, int64_t x_stride_t, int64_t x_stride_h, const int64_t* positions,
+                     const float* table, int table_rows, int T, int H, int d_r, int dtype, int interleaved,
+                     int inverse, void* out, int64_t o_stride_t, int64_t o_stride_h, void* stream);
+
+/* The absorbed form over the paged cache. Query (b, t, h) of q [B][Tq][H][d_c + d_r] sees the cache
+ * rows j < seq_lens[b] - Tq + t + 1 of sequence b (its last Tq rows are the queries' own tokens),
+ * row j at page block_table[b][j / page_size], offset j % page_size:
+ *   s_j = scale * q . row_j,  p = softmax(s),  out [B][Tq][H][d_c] = sum_j p_j row_j[0 .. d_c),
+ *   lse [B][Tq][H] = log sum_j exp(s_j); a query that sees nothing gets zeros and -inf.
+ * d_c 128, 256, 384 or 512; d_r 0 or 64; page_size a multiple of 8. out and lse contiguous.
+ * Workspace of ll_paged_latent_workspace_bytes, needed until the call's kernels have run. */
+size_t ll_paged_latent_workspace_bytes(int B, int Tq, int H, int d_c);
+int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
+                              const void* cache, int64_t page_stride, int64_t row_stride, int pages, int page_size,
+                              const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
+                              int B, int Tq, int H, int d_c, int d_r, float scale, int dtype, void* out, float* lse,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/* The expanded form on packed sequences: queries q [Tq][H][d_n + d_r], keys k_nope [Tk][H][d_n]
+ * beside the shared k_pe [Tk][d_r], values v [Tk][H][d_v]; sequence b holds query rows cu_q[b] ..
+ * cu_q[b + 1] and key rows cu_k[b] .. cu_k[b + 1] (int32 [B + 1], device). With causal, query i of
+ * a sequence sees its keys j <= i + (keys - queries), else all of them. d_n and d_v 64 or 128, d_r
+ * 0 or 64. */
+typedef struct {
+  int B, Tq, Tk, H, d_n, d_r, d_v;
+  int causal, dtype;
+  float scale;
+  const void* q;      int64_t q_stride_t, q_stride_h;
+  const void* k_nope; int64_t k_stride_t, k_stride_h;
+  const void* k_pe;   int64_t kpe_stride_t;
+  const void* v;      int64_t v_stride_t, v_stride_h;
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+} ll_latent_packed;
+
+/* out [Tq][H][d_v] and lse [H][Tq] (natural logarithm; a query that sees nothing: zeros and -inf). */
+int ll_latent_forward(const ll_latent_packed* a, void* out, float* lse, void* stream);
+
+/* Gradients of the forward for the gradient g of out [Tq][H][d_v] (strides given), from its out and
+ * lse: dq [Tq][H][d_n + d_r], dk_nope [Tk][H][d_n], dk_pe [Tk][d_r] (summed over the heads in 32
+ * bits, in a fixed order), dv [Tk][H][d_v], contiguous, written whole. Deterministic. */
+size_t ll_latent_backward_workspace_bytes(const ll_latent_packed* a);
+int ll_latent_backward(const ll_latent_packed* a, const void* g, int64_t g_stride_t, int64_t g_stride_h,
+                       const void* out, const float* lse, void* dq, void* dk_nope, void* dk_pe, void* dv,
+                       void* workspace, size_t workspace_bytes, void* stream);
+
+/* One product per head: y[t][h] = x[t][h] . W[h], bf16 with fp32 accumulation; W[h] is [N][K] (w_nk
+ * 1, y = x W^T) or [K][N] (0), w_stride_h apart with leading dimension ldw. */
+int ll_gemm_bf16_heads(int T, int H, int N, int K, const void* x, int64_t x_stride_t, int64_t x_stride_h,
+                       const void* W, int64_t w_stride_h, int64_t ldw, int w_nk, void* y, int64_t y_stride_t,
+                       int64_t y_stride_h, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

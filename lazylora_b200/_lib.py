@@ -45,6 +45,19 @@ class MoELayerDesc(ctypes.Structure):
     ]
 
 
+class LatentPacked(ctypes.Structure):
+    """Mirror of ll_latent_packed."""
+    _fields_ = [
+        ("B", c_int), ("Tq", c_int), ("Tk", c_int), ("H", c_int), ("d_n", c_int), ("d_r", c_int), ("d_v", c_int),
+        ("causal", c_int), ("dtype", c_int), ("scale", c_float),
+        ("q", c_void_p), ("q_stride_t", c_int64), ("q_stride_h", c_int64),
+        ("k_nope", c_void_p), ("k_stride_t", c_int64), ("k_stride_h", c_int64),
+        ("k_pe", c_void_p), ("kpe_stride_t", c_int64),
+        ("v", c_void_p), ("v_stride_t", c_int64), ("v_stride_h", c_int64),
+        ("cu_q", c_void_p), ("cu_k", c_void_p),
+    ]
+
+
 _SIGS = {
     "ll_status_string": (ctypes.c_char_p, [c_int]),
     "ll_last_cuda_error": (ctypes.c_char_p, []),
@@ -111,6 +124,22 @@ _SIGS = {
                                   c_void_p, c_int, ctypes.c_int64, c_void_p, ctypes.c_int64, c_int, c_void_p,
                                   ctypes.c_int64, c_int, c_void_p]),
     "ll_gemm_bf16_status": (c_int, [c_void_p]),
+    "ll_gemm_bf16_heads": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+                                   c_int, c_void_p, c_int64, c_int64, c_void_p]),
+    "ll_latent_status": (c_int, [c_void_p]),
+    "ll_latent_append": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                 c_int, c_void_p, c_int64, c_int64, c_int, c_int, c_void_p, c_int64, c_int64, c_int,
+                                 c_void_p, c_int64, c_int64, c_void_p]),
+    "ll_latent_rotate": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                 c_int, c_int, c_void_p, c_int64, c_int64, c_void_p]),
+    "ll_paged_latent_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "ll_paged_latent_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int,
+                                          c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
+                                          c_float, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "ll_latent_forward": (c_int, [ctypes.POINTER(LatentPacked), c_void_p, c_void_p, c_void_p]),
+    "ll_latent_backward_workspace_bytes": (c_size_t, [ctypes.POINTER(LatentPacked)]),
+    "ll_latent_backward": (c_int, [ctypes.POINTER(LatentPacked), c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                                   c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ll_rmsnorm_forward": (c_int, [c_void_p, c_void_p, c_int, c_int, ctypes.c_float, c_void_p, c_int, c_void_p,
                                    c_void_p]),
     "ll_rmsnorm_backward": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p]),

@@ -47,6 +47,7 @@ struct DenseArgs {
   int M, N, BN, mt, S, stage_bytes;
   int n_jobs, tiles0, tiles;   // tiles of job 0, all tiles
   int c_bf16;
+  int64_t c_head;              // elements between the heads' outputs (per-head products)
   DenseJob job[2];
 };
 
@@ -70,6 +71,10 @@ LL_DEV uint32_t idesc_bf16_m128_major(uint32_t n, bool b_mn_major) {
   return d;
 }
 
+// HEADS: one product per head, C[:, h] = A[:, h] . op(B[h]). The tensor maps have the head as a third
+// dimension and the tiles of a head follow one another (M fastest), so a head's weight stays in L2 for
+// its tiles; everything else is the single-job GEMM.
+template <bool HEADS>
 __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_constant__ DenseTma tm, const DenseArgs args) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -106,9 +111,10 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
   pdl_launch_next();                        // (after the allocation)
   pdl_wait();
 
-  auto tile_of = [&](int u, int& j, int& m0, int& n0) {
-    j = u < args.tiles0 ? 0 : 1;
-    const int v = j ? u - args.tiles0 : u;
+  auto tile_of = [&](int u, int& j, int& m0, int& n0, int& hd) {
+    j = HEADS || u < args.tiles0 ? 0 : 1;
+    hd = HEADS ? u / args.tiles0 : 0;           // tiles0: the tiles of a head
+    const int v = HEADS ? u % args.tiles0 : j ? u - args.tiles0 : u;
     m0 = (v % args.mt) * 128;
     n0 = (v / args.mt) * BN;
   };
@@ -121,8 +127,8 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
       bool ok = true;
       const uint32_t tx = kDnAStage + BN * kDnBK * 2;
       for (int u = blockIdx.x; u < args.tiles && ok; u += gridDim.x) {
-        int j, m0, n0;
-        tile_of(u, j, m0, n0);
+        int j, m0, n0, hd;
+        tile_of(u, j, m0, n0, hd);
         const DenseJob& jb = args.job[j];
         for (int p = 0; p < jb.n_pairs && ok; p++) {
           const CUtensorMap* am = &tm.a[jb.map[p]];
@@ -132,11 +138,22 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
             uint8_t* a_s = stages + s * STG;
             uint8_t* b_s = a_s + kDnAStage;
             mbar_arrive_expect_tx(&full[s], tx);
-            tma_load_2d(a_s, am, &full[s], kb * kDnBK, m0);
-            if (!jb.b_mn[p]) {
-              tma_load_2d(b_s, bm, &full[s], kb * kDnBK, n0);
+            if (HEADS) {
+              tma_load_3d(a_s, am, &full[s], kb * kDnBK, m0, hd);
+              if (!jb.b_mn[p]) {
+                tma_load_3d(b_s, bm, &full[s], kb * kDnBK, n0, hd);
+              } else {
+                for (int c = 0; c < BN / 64; c++)
+                  tma_load_3d(b_s + c * 64 * 128, bm, &full[s], n0 + 64 * c, kb * kDnBK, hd);
+              }
             } else {
-              for (int c = 0; c < BN / 64; c++) tma_load_2d(b_s + c * 64 * 128, bm, &full[s], n0 + 64 * c, kb * kDnBK);
+              tma_load_2d(a_s, am, &full[s], kb * kDnBK, m0);
+              if (!jb.b_mn[p]) {
+                tma_load_2d(b_s, bm, &full[s], kb * kDnBK, n0);
+              } else {
+                for (int c = 0; c < BN / 64; c++)
+                  tma_load_2d(b_s + c * 64 * 128, bm, &full[s], n0 + 64 * c, kb * kDnBK);
+              }
             }
             issued++;
             if (++s == S) { s = 0; ph ^= 1; }
@@ -155,8 +172,8 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
       uint32_t ev = 0;
       bool ok = true;
       for (int u = blockIdx.x; u < args.tiles && ok; u += gridDim.x) {
-        int j, m0, n0;
-        tile_of(u, j, m0, n0);
+        int j, m0, n0, hd;
+        tile_of(u, j, m0, n0, hd);
         const DenseJob& jb = args.job[j];
         if (!(ok = seq_wait(ready_seq, ++ev, abort_flag, st, 43))) break;   // accumulator ab drained
         tc_fence_after();
@@ -198,8 +215,8 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
       int s = 0, ab = 0;
       uint32_t ph = 0, abph = 0, ev = 0;
       for (int u = blockIdx.x; u < args.tiles; u += gridDim.x) {
-        int j, m0, n0;
-        tile_of(u, j, m0, n0);
+        int j, m0, n0, hd;
+        tile_of(u, j, m0, n0, hd);
         const DenseJob& jb = args.job[j];
         mbar_wait(&accempty[ab], abph ^ 1, abort_flag, st, 46);
         seq_publish(ready_seq, ++ev);
@@ -220,8 +237,8 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
     uint32_t abph = 0;
     bool ok = true;
     for (int u = blockIdx.x; u < args.tiles && ok; u += gridDim.x) {
-      int j, m0, n0;
-      tile_of(u, j, m0, n0);
+      int j, m0, n0, hd;
+      tile_of(u, j, m0, n0, hd);
       const DenseJob& jb = args.job[j];
       if (!(ok = mbar_wait_sleep(&accfull[ab], abph, abort_flag, st, 48, 512))) break;
       tc_fence_after();
@@ -234,7 +251,7 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
         const int col = n0 + c;
         if (row >= args.M || col >= args.N) continue;
         if (args.c_bf16) {
-          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(jb.C) + (int64_t)row * jb.ldc + col;
+          __nv_bfloat16* out = static_cast<__nv_bfloat16*>(jb.C) + (HEADS ? hd * args.c_head : 0) + (int64_t)row * jb.ldc + col;
           if (col + 16 <= args.N) {
             uint4 w[2];
             uint32_t* wp = reinterpret_cast<uint32_t*>(w);
@@ -643,9 +660,48 @@ static int dense_gemm(int M, int N, int n_jobs, const int* pairs_per_job, const 
     const int grid = 2 * std::min(a.tiles, units);
     return launch_pdl("k_dense_gemm_pair", k_dense_gemm_pair, dim3(grid), dim3(kDnThreads), smem, s, tm, a);
   }
-  LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_dense_gemm), smem));
+  LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_dense_gemm<false>), smem));
   const int grid = std::min(a.tiles, di.sms);
-  return launch_pdl("k_dense_gemm", k_dense_gemm, dim3(grid), dim3(kDnThreads), smem, s, tm, a);
+  return launch_pdl("k_dense_gemm", k_dense_gemm<false>, dim3(grid), dim3(kDnThreads), smem, s, tm, a);
+}
+
+// y[:, h] = x[:, h] . op(W[h]) for every head, on the single-CTA kernel.
+static int head_gemm(int T, int H, int N, int K, const void* x, int64_t x_t, int64_t x_h, const void* W, int64_t w_h,
+                     int64_t ldw, int w_nk, void* y, int64_t y_t, int64_t y_h, cudaStream_t s) {
+  const DeviceInfo di = device_info();
+  DenseArgs a{};
+  a.M = T;
+  a.N = N;
+  a.BN = pick_bn(T, N, H, !w_nk, di.sms, false);
+  a.mt = (T + 127) / 128;
+  a.stage_bytes = kDnAStage + a.BN * kDnBK * 2;
+  a.S = std::min(kDnMaxStages, (kDnSmemBudget - 1024 - 1024) / a.stage_bytes);
+  a.n_jobs = 1;
+  a.c_bf16 = 1;
+  a.c_head = y_h;
+  DenseJob& jb = a.job[0];
+  jb.C = y;
+  jb.ldc = y_t;
+  jb.n_pairs = 1;
+  jb.nt = (N + a.BN - 1) / a.BN;
+  jb.kb[0] = (K + kDnBK - 1) / kDnBK;
+  jb.b_mn[0] = w_nk ? 0 : 1;
+  DenseTma tm;
+  const uint64_t xd[3] = {(uint64_t)K, (uint64_t)T, (uint64_t)H}, xs[2] = {(uint64_t)x_t * 2, (uint64_t)x_h * 2};
+  const uint32_t xb[3] = {kDnBK, 128, 1};
+  const uint64_t wd[3] = {(uint64_t)(w_nk ? K : N), (uint64_t)(w_nk ? N : K), (uint64_t)H};
+  const uint64_t ws[2] = {(uint64_t)ldw * 2, (uint64_t)w_h * 2};
+  const uint32_t wb[3] = {64, (uint32_t)(w_nk ? a.BN : kDnBK), 1};
+  LL_TRY(make_map_nd(&tm.a[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, x, 3, xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B));
+  LL_TRY(make_map_nd(&tm.b[0], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, W, 3, wd, ws, wb, CU_TENSOR_MAP_SWIZZLE_128B));
+  tm.a[1] = tm.a[0];
+  tm.b[1] = tm.b[0];
+  a.tiles0 = a.mt * jb.nt;
+  a.tiles = a.tiles0 * H;
+  const int smem = 1024 + 1024 + a.S * a.stage_bytes;
+  LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_dense_gemm<true>), smem));
+  const int grid = std::min(a.tiles, di.sms);
+  return launch_pdl("k_dense_gemm heads", k_dense_gemm<true>, dim3(grid), dim3(kDnThreads), smem, s, tm, a);
 }
 
 }  // namespace ll
@@ -692,6 +748,23 @@ int ll_gemm_bf16_sum2(int M, int N, const void* A0, int K0, int64_t lda0, const 
   void* const cs[1] = {C};
   const int64_t lc[1] = {ldc};
   return dense_gemm(M, N, 1, pairs, ops, cs, lc, c_dtype, s);
+}
+
+int ll_gemm_bf16_heads(int T, int H, int N, int K, const void* x, int64_t x_stride_t, int64_t x_stride_h,
+                       const void* W, int64_t w_stride_h, int64_t ldw, int w_nk, void* y, int64_t y_stride_t,
+                       int64_t y_stride_h, void* stream) {
+  if (T < 0 || H < 0 || N <= 0 || K <= 0 || ldw < (w_nk ? K : N)) return LL_ERR_ARG;
+  if (T == 0 || H == 0) return LL_OK;
+  if (!x || !W || !y) return LL_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(y)) % 16)
+    return LL_ERR_ARG;
+  if (x_stride_t % 8 || x_stride_h % 8 || w_stride_h % 8 || ldw % 8 || y_stride_t % 8 || y_stride_h % 8) return LL_ERR_ARG;
+  if (x_stride_t < K || x_stride_h < 8 || w_stride_h < 8 || y_stride_t < N || (H > 1 && y_stride_h < 8)) return LL_ERR_ARG;
+  if ((int64_t)((T + 127) / 128) * ((N + 31) / 32) * H > INT32_MAX) return LL_ERR_ARG;
+  LL_TRY(check_arch());
+  LL_STREAM(stream);
+  g_launch_count = 0;
+  return head_gemm(T, H, N, K, x, x_stride_t, x_stride_h, W, w_stride_h, ldw, w_nk, y, y_stride_t, y_stride_h, s);
 }
 
 int ll_gemm_bf16_status(void* stream) {
