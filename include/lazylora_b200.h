@@ -394,11 +394,12 @@ int ll_latent_rotate(const void* x, int64_t x_stride_t, int64_t x_stride_h, cons
  * row j at page block_table[b][j / page_size], offset j % page_size:
  *   s_j = scale * q . row_j,  p = softmax(s),  out [B][Tq][H][d_c] = sum_j p_j row_j[0 .. d_c),
  *   lse [B][Tq][H] = log sum_j exp(s_j); a query that sees nothing gets zeros and -inf.
- * d_c 128, 256, 384 or 512; d_r 0 or 64; page_size a multiple of 8. out and lse contiguous.
+ * Query row t * H + h of sequence b starts at b * q_stride_b + (t * H + h) * q_stride_row. d_c 128,
+ * 256, 384 or 512; d_r 0 or 64; page_size a multiple of 8. out and lse contiguous.
  * Workspace of ll_paged_latent_workspace_bytes, needed until the call's kernels have run. */
 size_t ll_paged_latent_workspace_bytes(int B, int Tq, int H, int d_c);
-int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
-                              const void* cache, int64_t page_stride, int64_t row_stride, int pages, int page_size,
+int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_stride_row, const void* cache,
+                              int64_t page_stride, int64_t row_stride, int pages, int page_size,
                               const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
                               int B, int Tq, int H, int d_c, int d_r, float scale, int dtype, void* out, float* lse,
                               void* workspace, size_t workspace_bytes, void* stream);

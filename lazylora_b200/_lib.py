@@ -133,7 +133,7 @@ _SIGS = {
     "ll_latent_rotate": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                  c_int, c_int, c_void_p, c_int64, c_int64, c_void_p]),
     "ll_paged_latent_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
-    "ll_paged_latent_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int,
+    "ll_paged_latent_attention": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int, c_int,
                                           c_void_p, c_int64, c_int, c_void_p, c_int, c_int, c_int, c_int, c_int,
                                           c_float, c_int, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "ll_latent_forward": (c_int, [ctypes.POINTER(LatentPacked), c_void_p, c_void_p, c_void_p]),

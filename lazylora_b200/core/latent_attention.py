@@ -156,14 +156,16 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
         raise ValueError("block_table: int32 [B, max_pages]")
     seq_lens = _ints(seq_lens, torch.int32, (B,), "seq_lens")
     lib, src = L.load(), _in(q)
+    if Tq > 1 and H > 1 and src.stride(1) != H * src.stride(2):     # the rows (t, h) must be evenly spaced
+        src = src.contiguous()
     out = torch.empty((B, Tq, H, d_c), dtype=q.dtype, device=q.device)
     lse = torch.empty((B, Tq, H), dtype=torch.float32, device=q.device)
     if out.numel() == 0:
         return out, lse
     n = lib.ll_paged_latent_workspace_bytes(B, Tq, H, d_c)
     ws = torch.empty(n, dtype=torch.uint8, device=q.device)
-    L.check(lib.ll_paged_latent_attention(src.data_ptr(), _st(src, 0), _st(src, 1), _st(src, 2), cache.data_ptr(),
-                                          _st(cache, 0), _st(cache, 1), cache.shape[0], cache.shape[1],
+    L.check(lib.ll_paged_latent_attention(src.data_ptr(), _st(src, 0), _st(src, 2) if H > 1 else _st(src, 1),
+                                          cache.data_ptr(), _st(cache, 0), _st(cache, 1), cache.shape[0], cache.shape[1],
                                           block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
                                           seq_lens.data_ptr(), B, Tq, H, d_c, d_r, float(scale), dt, out.data_ptr(),
                                           lse.data_ptr(), ws.data_ptr(), n, L.stream_ptr()),

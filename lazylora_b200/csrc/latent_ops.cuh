@@ -37,6 +37,58 @@ struct Num<__half> {
   }
 };
 
+// kind::f16 instruction descriptor: operands of format fmt (0 fp16, 1 bf16), fp32 accumulation.
+LL_DEV uint32_t idesc_16bit(uint32_t fmt, uint32_t m, uint32_t n, bool a_mn, bool b_mn) {
+  return 1u << 4 | fmt << 7 | fmt << 10 | (a_mn ? 1u : 0u) << 15 | (b_mn ? 1u : 0u) << 16 | (n >> 3) << 17 | (m >> 4) << 24;
+}
+
+// One lane of a converged warp.
+LL_DEV bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// A shared-memory operand descriptor (128-byte swizzle) as its two words: steps along the operand are
+// additions to lo, in units of 16 bytes (shared addresses stay below 2^18, so the field never carries).
+struct MmaDesc {
+  uint32_t lo, hi;
+  LL_DEV MmaDesc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
+    const uint64_t d = umma_desc(addr, lbo, sbo, kSwizzle128B);
+    lo = (uint32_t)d;
+    hi = (uint32_t)(d >> 32);
+  }
+};
+
+// D[tmem] (+)= A B, kind::f16, both operands in shared memory.
+LL_DEV void mma_16bit(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc,
+                      uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\t"
+      "mov.b64 x, {%1, %2};\n\tmov.b64 y, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The same with A in tensor memory.
+LL_DEV void mma_16bit_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\t"
+      "mov.b64 y, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// 2^x (ex2.approx: 2 ulp, results below the normal range to zero).
+LL_DEV float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // Rows of sequence b in a packed tensor of `total` rows: [lo, hi), clamped into the tensor so that
 // no value of cu can lead outside it.
 LL_DEV void seq_range(const int32_t* cu, int b, int total, int& lo, int& hi) {

@@ -1,87 +1,585 @@
 // The absorbed form of latent attention over a paged cache (see the header for the interface): all
-// rows of a sequence's queries read the same cache rows, which are keys (all d_c + d_r values) and
-// values (the first d_c) at once.
-//   s_j = scale q . row_j,  m = max_j s_j,  p_j = exp(s_j - m),  l = sum_j p_j,
-//   out = (sum_j p_j row_j[:d_c]) / l,  lse = m + log l.
-// First form: one block per (sequence, 16 query rows), each warp two rows, a lane per key of a
-// 32-key tile, running maximum and sum; CUDA cores throughout.
+// rows (t, h) of a sequence's queries read the same cache rows, which are keys (all d_c + d_r values)
+// and values (the first d_c) at once.
+//   s_j = scale q . row_j,  p_j = 2^(s_j log2 e - m),  l = sum_j p_j,
+//   out = (sum_j p_j row_j[:d_c]) / l,  lse = (m + log2 l) ln 2  for any reference m.
+//
+// Bound by HBM up to about 128 query rows (1152 bytes a key against 2 * 1088 flops a key and row).
+// Both products are therefore taken transposed, with the cache rows as the tall operand A and the
+// query rows as N, so that the tensor cores' work follows the number of rows instead of a padded
+// 128, and one copy of a key tile in shared memory serves both:
+//   S^T [64 keys][NT rows]  = tile (K-major) . Q^T       M = 64,  K = d_c + d_r
+//   O^T [d_c][NT rows]     += tile^T (MN-major) . P^T    M = 128 (d_c / 128 times), K = 64 keys
+// with NT = 16 .. 64 rows a CTA (more rows: more CTAs that read the same tiles, through L2, at the
+// same time). O^T takes d_c / 128 * NT columns of tensor memory, S^T two times 64.
+//
+// A key tile lies in shared memory as eight groups of eight rows, [group][64-column chunk][8 rows][128
+// bytes] with the 128-byte swizzle: one TMA box per group, so any page size that is a multiple of 8
+// works and no page boundary lies inside a box, and a uniform group stride for both operand forms.
+//
+// Softmax: a thread owns one key and half of the rows, S^T's tensor-memory lanes being keys. The
+// reference m of a row only has to be within 2^8 of its running maximum, so a tile first asks (one
+// barrier with a vote) whether any score passes its reference by more than 8; only then are the maxima
+// taken across the keys, and O^T and l rescaled. l stays a partial sum per thread until the end. P is
+// rounded to the 16-bit type for the tensor cores (2^-9 or 2^-12 relative, as the output's own
+// rounding); l sums the unrounded values in fp32.
+//
+// The tiles of all sequences, one after another, are dealt to the CTAs in equal contiguous ranges
+// (from the lengths on the device, so a captured graph may be replayed with other lengths). A CTA whose
+// range covers a sequence writes its output; pieces of a sequence go to the workspace (O in fp32, m, l)
+// and k_paged_combine joins them in order. Six warps: 0-3 softmax, rescaling, outputs; 4 TMA; 5 MMA.
+//
+// Rows of the last tile past the sequence's end, which may hold anything, are set to zero in shared
+// memory before the second product (0 * NaN would reach the sums) and masked by their index.
 #include "latent_ops.cuh"
 
 namespace ll {
 
+constexpr int kPgThreads = 192;
+constexpr int kPgKeys = 64;
+constexpr float kPgSlack = 8.f;        // log2 of how far a score may pass its row's reference
+constexpr float kPgNone = -1e30f;      // reference of a row that has seen no key
+
 struct PagedArgs {
-  const void* q;
-  const void* cache;
   const int32_t* bt;
   const int32_t* lens;
   void* out;
   float* lse;
-  int64_t q_b, q_t, q_h, page_stride, row_stride, bt_stride;
-  int pages, page_size, max_pages, Tq, H, d_c, d_r;
-  float scale;
+  float* part;        // [G * 2][RT][NT][d_c] unnormalised pieces
+  float* part_ml;     // [G * 2][RT][2][NT] their references (log2) and sums
+  int64_t* starts;    // [B + 1] tiles before each sequence; last: tiles of a range
+  int64_t bt_stride;
+  int pages, page_size, max_pages, B, Tq, H, rows, RT, G, nc, nchunk;   // chunks of 64: of d_c, of d_c + d_r
+  float scale_log2;
   DevStatus* st;
 };
 
+struct PagedTma {
+  CUtensorMap q, kv;
+};
+
+LL_DEV int paged_len(const PagedArgs& a, int b) {
+  return (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page_size);
+}
+// A sequence without keys still has one (masked) tile, which writes its zeros.
+LL_DEV int paged_tiles(int len) { return max(1, (len - 1) / kPgKeys + 1); }
+
+// tcgen05.ld of 16 lanes x 8 columns twice: threads 0-15 take columns taddr .. + 7, threads 16-31
+// columns taddr + SPLIT .. + 7 of the same lanes.
+template <int SPLIT>
+LL_DEV void tmem_ld_16x2_8(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8], %9;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr), "n"(SPLIT));
+}
+
+// A softmax thread's NH values of S^T.
+template <int NH>
+LL_DEV void load_scores(uint32_t taddr, float (&v)[NH]) {
+  uint32_t raw[NH];
+#pragma unroll
+  for (int c = 0; c < NH; c += 8) tmem_ld_16x2_8<NH>(taddr + c, raw + c);
+  tmem_ld_wait();
+#pragma unroll
+  for (int c = 0; c < NH; c += 8)
+    asm volatile("" : "+r"(raw[c]), "+r"(raw[c + 1]), "+r"(raw[c + 2]), "+r"(raw[c + 3]), "+r"(raw[c + 4]),
+                 "+r"(raw[c + 5]), "+r"(raw[c + 6]), "+r"(raw[c + 7])::"memory");
+#pragma unroll
+  for (int c = 0; c < NH; c++) v[c] = __uint_as_float(raw[c]);
+}
+
+// Folds N values a thread across the 16 lanes of its half warp, halving the values a lane carries at each
+// step instead of repeating every value in every lane (30 shuffles for 32 values instead of 128). Returns
+// the first of the fold_left(N) value indexes that this lane ends up with.
+constexpr int fold_left(int n) {
+  for (int i = 0; i < 4; i++) n = n % 2 == 0 ? n / 2 : n;
+  return n;
+}
+template <int N, int OFF, class Op>
+LL_DEV int fold16(float* v, int lane, Op op) {
+  if constexpr (OFF == 0) {
+    return 0;
+  } else if constexpr (N % 2 == 0) {
+    const bool up = lane & OFF;
+#pragma unroll
+    for (int i = 0; i < N / 2; i++) {
+      const float got = __shfl_xor_sync(0xffffffffu, up ? v[i] : v[i + N / 2], OFF);
+      v[i] = op(up ? v[i + N / 2] : v[i], got);
+    }
+    return (up ? N / 2 : 0) + fold16<N / 2, OFF / 2>(v, lane, op);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) v[i] = op(v[i], __shfl_xor_sync(0xffffffffu, v[i], OFF));
+    return fold16<N, OFF / 2>(v, lane, op);
+  }
+}
+
+// Barrier 1 of the 128 softmax threads, with a vote.
+LL_DEV bool softmax_any(bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)p)
+      : "memory");
+  return r != 0;
+}
+
+// The pieces [j, j_end) of sequence b, one after another, that make up a CTA's range of tiles.
+struct PagedWalk {
+  int64_t left;
+  int b, j, n, len;
+  LL_DEV void init(const PagedArgs& a, int b0, int j0, int64_t count) {
+    left = count;
+    b = b0;
+    j = j0;
+    if (left > 0) set(a);
+  }
+  LL_DEV void set(const PagedArgs& a) {
+    len = paged_len(a, b);
+    n = paged_tiles(len);
+  }
+  LL_DEV int end() const { return (int)min((int64_t)n, j + left); }
+  LL_DEV void next(const PagedArgs& a) {
+    left -= end() - j;
+    b++;
+    j = 0;
+    if (left > 0) set(a);
+  }
+};
+
+template <class T, int NT>
+__global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__ PagedTma tm, const PagedArgs a) {
+  constexpr int NH = NT / 2;             // rows of a softmax thread
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nchunk = a.nchunk, group_bytes = nchunk * 1024, tile_bytes = 8 * group_bytes;
+  uint8_t* s_kv = base;                               // two tiles
+  uint8_t* s_q = s_kv + 2 * tile_bytes;               // [chunk][NT rows][128 bytes]
+  uint8_t* s_p = s_q + nchunk * NT * 128;             // [64 keys][128 bytes]: P^T, rows of NT values
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_p + kPgKeys * 128);
+  uint64_t *kv_full = bars, *kv_empty = bars + 2, *s_full = bars + 4, *q_full = bars + 6, *q_empty = bars + 7,
+           *p_ready = bars + 8, *pv_done = bars + 9, *o_free = bars + 10, *drain = bars + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_start = reinterpret_cast<int*>(tmem_slot + 2);                // b0, j0, count, per
+  float* s_red = reinterpret_cast<float*>(tmem_slot + 8);              // [4 warps][64]
+  float* s_col = s_red + 256;                                          // [64] a factor per row
+  float* s_ref = s_col + 64;                                           // [64] the rows' references
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int g = blockIdx.x / a.RT, rt = blockIdx.x % a.RT;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 12; i++) mbar_init(&bars[i], i == 8 || i == 10 ? 4 : 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) tmem_alloc(tmem_slot, 512);
+  if (warp == 4 && lane == 0) {
+    tma_prefetch_desc(&tm.q);
+    tma_prefetch_desc(&tm.kv);
+  }
+  pdl_wait();
+  if (warp == 0) {
+    // the range of this CTA: each lane sums a run of consecutive sequences
+    const int run = (a.B + 31) / 32, b_lo = min(lane * run, a.B), b_hi = min(b_lo + run, a.B);
+    int64_t mine = 0;
+    for (int b = b_lo; b < b_hi; b++) mine += paged_tiles(paged_len(a, b));
+    int64_t sum = mine;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, sum, off);
+      if (lane >= off) sum += v;
+    }
+    const int64_t total = __shfl_sync(0xffffffffu, sum, 31), per = (total + a.G - 1) / a.G, first = g * per;
+    if (lane == 0) s_start[2] = (int)max((int64_t)0, min(per, total - first));
+    if (blockIdx.x == 0) {
+      int64_t at = sum - mine;
+      for (int b = b_lo; b < b_hi; b++) {
+        a.starts[b] = at;
+        at += paged_tiles(paged_len(a, b));
+      }
+      if (lane == 0) a.starts[a.B] = per;
+    }
+    if (first >= sum - mine && first < sum) {
+      int64_t at = sum - mine;
+      int b = b_lo;
+      for (int n; at + (n = paged_tiles(paged_len(a, b))) <= first; b++) at += n;
+      s_start[0] = b;
+      s_start[1] = (int)(first - at);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_next();
+  const uint32_t tmem = *tmem_slot, tmem_s = tmem + 256;
+  const int count = s_start[2];
+  PagedWalk w;
+  w.init(a, s_start[0], s_start[1], count);
+
+  if (warp == 4) {
+    // ------------------------------------------------------------------------------- TMA
+    // Lane i takes the tile's group i of eight keys: it looks its page up while the stage is still in
+    // use, then issues its own box.
+    bool ok = true;
+    uint32_t n = 0, seg = 0, q_loads = 0;
+    for (; w.left > 0 && ok; w.next(a), seg++) {
+      const int j0 = w.j, j1 = w.end();
+      for (int j = j0; j < j1; j++, n++) {
+        const int st = n & 1, key = j * kPgKeys + lane * 8;
+        const int groups = (min(kPgKeys, max(0, w.len - j * kPgKeys)) + 7) / 8;
+        int page = a.pages;                       // outside the map: reads zeros
+        if (lane < groups) {
+          const int at = key / a.page_size, id = a.bt[w.b * a.bt_stride + at];
+          if (id >= 0 && id < a.pages) page = id;
+          else report(a.st, LL_ERR_RANGE, 73, w.b);
+        }
+        const int off = key % a.page_size;
+        if (lane == 0) {
+          ok = mbar_wait(&kv_empty[st], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 81);
+          if (ok) mbar_arrive_expect_tx(&kv_full[st], groups * group_bytes);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        if (!ok) break;
+        if (lane < groups) tma_load_4d(s_kv + st * tile_bytes + lane * group_bytes, &tm.kv, &kv_full[st], 0, off, 0, page);
+        if (j == j0) {
+          if (lane == 0) {
+            ok = mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, a.st, 82);
+            if (ok) mbar_arrive_expect_tx(q_full, nchunk * NT * 128);
+          }
+          ok = __shfl_sync(0xffffffffu, ok, 0);
+          if (!ok) { n++; break; }
+          q_loads++;
+          if (lane < nchunk) tma_load_3d(s_q + lane * NT * 128, &tm.q, q_full, lane * 64, rt * NT, w.b);
+        }
+      }
+    }
+    volatile int keep = 0;                        // what was issued has landed, also after an abort
+    if (n >= 1) mbar_wait_sleep(&kv_full[(n - 1) & 1], ((n - 1) >> 1) & 1, &keep, a.st, 83, 64);
+    if (n >= 2) mbar_wait_sleep(&kv_full[n & 1], ((n - 2) >> 1) & 1, &keep, a.st, 84, 64);
+    if (q_loads >= 1) mbar_wait_sleep(q_full, (q_loads - 1) & 1, &keep, a.st, 85, 64);
+    __syncwarp();
+  } else if (warp == 5) {
+    // ------------------------------------------------------------------------------- MMA
+    // The whole warp runs the loop (so that descriptors stay in uniform registers), one elected
+    // lane issues. S^T of tile n + 1 goes ahead of tile n's second product when its tile has already
+    // landed, and behind it otherwise: with two tiles in flight, waiting for a tile while a second
+    // product could run would hold up the very stage that the next tile is to land in.
+    const bool lead = elect_one();
+    const uint32_t id_s = idesc_16bit(Num<T>::fmt, 64, NT, false, false);
+    const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, NT, true, true);
+    const MmaDesc q_d(smem_u32(s_q), 16, 1024), p_d(smem_u32(s_p), 1024, 1024);
+    const MmaDesc k_d(smem_u32(s_kv), 16, group_bytes), v_d(smem_u32(s_kv), 1024, group_bytes);
+    const uint32_t tile16 = tile_bytes >> 4, group16 = group_bytes >> 4;
+    const int mts = a.nc / 2;
+    uint32_t qk = 0, pv = 0, seg = 0, seg_pv = 0, first_bits = 0;   // first_bits: tile is its piece's first
+    int j = w.j;
+    long long t0 = clock64();
+    while (pv < (uint32_t)count) {
+      bool did = false;
+      if (qk < (uint32_t)count && qk - pv <= 1 && mbar_try_wait(&kv_full[qk & 1], (qk >> 1) & 1) &&
+          (j != w.j || mbar_try_wait(q_full, seg & 1))) {
+        tc_fence_after();
+        const uint32_t at = tmem_s + (qk & 1) * 64, k0 = k_d.lo + (qk & 1) * tile16;
+        if (lead) {
+          for (int c = 0; c < nchunk; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit(at, k0 + c * 64 + kk * 2, k_d.hi, q_d.lo + c * (NT * 8) + kk * 2, q_d.hi, id_s, c + kk);
+          mma_commit(&s_full[qk & 1]);
+          if (j == w.end() - 1) mma_commit(q_empty);
+        }
+        first_bits = (first_bits & ~(1u << (qk & 1))) | (j == w.j ? 1u : 0u) << (qk & 1);
+        qk++;
+        if (++j == w.end()) {
+          w.next(a);
+          j = w.j;
+          seg++;
+        }
+        did = true;
+      }
+      const bool first = first_bits >> (pv & 1) & 1;
+      if (pv < qk && mbar_try_wait(p_ready, pv & 1) && (!first || seg_pv == 0 || mbar_try_wait(o_free, (seg_pv - 1) & 1))) {
+        tc_fence_after();
+        const uint32_t v0 = v_d.lo + (pv & 1) * tile16;
+        if (lead) {
+#pragma unroll
+          for (int kk = 0; kk < kPgKeys / 16; kk++)
+#pragma unroll
+            for (int mt = 0; mt < 4; mt++)
+              if (mt < mts)
+                mma_16bit(tmem + mt * NT, v0 + kk * 2 * group16 + mt * 128, v_d.hi, p_d.lo + kk * 128, p_d.hi, id_o,
+                          first && kk == 0 ? 0 : 1);
+          mma_commit(&kv_empty[pv & 1]);
+          mma_commit(pv_done);
+        }
+        pv++;
+        // a piece's first tile opens the next piece's wait for its outputs
+        if (first) seg_pv++;
+        did = true;
+      }
+      if (did) t0 = clock64();
+      else if (*abort_flag) break;
+      else if (clock64() - t0 > kWaitLimitCycles) {
+        *abort_flag = 1;
+        if (lead) report(a.st, LL_ERR_TIMEOUT, 86, (int)pv);
+        break;
+      }
+    }
+    if (lead) mma_commit(drain);
+    volatile int keep = 0;
+    mbar_wait_sleep(drain, 0, &keep, a.st, 90, 64);
+    __syncwarp();
+  } else {
+    // ------------------------------------------------- softmax, rescaling and the outputs
+    // A wait that ran out does not leave the loops: the other waits then return at once, every
+    // barrier still meets all 128 threads, and the results are void (the status says so).
+    const int hh = lane / 16, key_in = warp * 16 + lane % 16;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const int t0 = (rt * NT + hh * NH) / a.H, h0 = (rt * NT + hh * NH) % a.H;
+    uint8_t* p_row = s_p + (key_in / 8) * 1024 + (key_in % 8) * 128;
+    uint32_t n = 0;
+    for (; w.left > 0; w.next(a)) {
+      const int j0 = w.j, j1 = w.end();
+      float ref[NH], l[NH];
+#pragma unroll
+      for (int c = 0; c < NH; c++) { ref[c] = kPgNone; l[c] = 0.f; }
+      if (threadIdx.x < NT) s_ref[threadIdx.x] = kPgNone;
+      for (int j = j0; j < j1; j++, n++) {
+        mbar_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.st, 91);
+        tc_fence_after();
+        const uint32_t s_at = tmem_s + (n & 1) * 64 + lanes;
+        const int k0 = j * kPgKeys, key = k0 + key_in;
+        const bool inside = k0 + kPgKeys <= w.len - a.Tq + 1;       // every row sees every key
+        // hides the keys past each row's last one (row (t, h) sees w.len - Tq + 1 + t of them)
+        auto mask = [&](float (&x)[NH]) {
+          int h = h0, see = w.len - a.Tq + 1 + t0;
+#pragma unroll
+          for (int c = 0; c < NH; c++) {
+            if (key >= see) x[c] = -INFINITY;
+            if (++h == a.H) { h = 0; see++; }
+          }
+        };
+        float v[NH];
+        load_scores<NH>(s_at, v);
+#pragma unroll
+        for (int c = 0; c < NH; c++) v[c] = fmaf(v[c], a.scale_log2, -ref[c]);
+        if (!inside) mask(v);
+        float top = v[0];
+#pragma unroll
+        for (int c = 1; c < NH; c++) top = fmaxf(top, v[c]);
+        const bool slow = softmax_any(top > kPgSlack);
+        if (slow) {
+          // new references: each row's maximum so far
+          load_scores<NH>(s_at, v);
+#pragma unroll
+          for (int c = 0; c < NH; c++) v[c] *= a.scale_log2;
+          if (!inside) mask(v);
+          float x[NH];
+#pragma unroll
+          for (int c = 0; c < NH; c++) x[c] = v[c];
+          const int c0 = hh * NH + fold16<NH, 8>(x, lane, [](float p, float q) { return fmaxf(p, q); });
+#pragma unroll
+          for (int c = 0; c < fold_left(NH); c++) s_red[warp * 64 + c0 + c] = x[c];
+          named_bar_sync(1, 128);
+          if (threadIdx.x < NT) {
+            const int r = threadIdx.x;
+            const float was = s_ref[r];
+            const float now = fmaxf(fmaxf(fmaxf(s_red[r], s_red[64 + r]), fmaxf(s_red[128 + r], s_red[192 + r])), was);
+            s_ref[r] = now;
+            s_col[r] = ex2(was - now);
+          }
+          named_bar_sync(1, 128);
+#pragma unroll
+          for (int c = 0; c < NH; c++) {
+            ref[c] = s_ref[hh * NH + c];
+            v[c] -= ref[c];
+            l[c] *= s_col[hh * NH + c];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < NH; c++) {
+          v[c] = ex2(v[c]);
+          l[c] += v[c];
+        }
+        if (n > 0) mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.st, 92);      // P and O are free
+        if (slow && j > j0) {
+          tc_fence_after();
+          for (int mt = 0; mt < a.nc / 2; mt++)
+            for (int c = 0; c < NT; c += 16) {
+              float o[16];
+              const uint32_t at = tmem + mt * NT + c + lanes;
+              tmem_ld16(at, o);
+              tmem_ld_wait();
+              uint32_t u[16];
+#pragma unroll
+              for (int i = 0; i < 16; i++) u[i] = __float_as_uint(o[i] * s_col[c + i]);
+              tmem_st16(at, u);
+            }
+          tmem_st_wait();
+        }
+#pragma unroll
+        for (int c = 0; c < NH; c += 8) {
+          const int chunk = (hh * NH + c) / 8;
+          *reinterpret_cast<uint4*>(p_row + ((chunk ^ (key_in % 8)) * 16)) =
+              make_uint4(Num<T>::pack(v[c], v[c + 1]), Num<T>::pack(v[c + 2], v[c + 3]), Num<T>::pack(v[c + 4], v[c + 5]),
+                         Num<T>::pack(v[c + 6], v[c + 7]));
+        }
+        const int valid = w.len - k0;
+        if (valid < kPgKeys) {
+          const int from = max(valid, 0), per_row = a.nc * 8;
+          for (int i = threadIdx.x; i < (kPgKeys - from) * per_row; i += 128) {
+            const int r = from + i / per_row, c = i % per_row;
+            *reinterpret_cast<uint4*>(s_kv + (n & 1) * tile_bytes + (r / 8) * group_bytes + (c / 8) * 1024 + (r % 8) * 128 +
+                                      (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_async_smem();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready);
+      }
+      // the piece's sums over its keys, in a fixed order
+      const int c0 = hh * NH + fold16<NH, 8>(l, lane, [](float p, float q) { return p + q; });
+#pragma unroll
+      for (int c = 0; c < fold_left(NH); c++) s_red[warp * 64 + c0 + c] = l[c];
+      named_bar_sync(1, 128);
+      const bool whole = j0 == 0 && j1 == w.n;
+      const int64_t slot = ((int64_t)g * 2 + (n == (uint32_t)(j1 - j0) ? 0 : 1)) * a.RT + rt;
+      if (threadIdx.x < NT) {
+        const int r = threadIdx.x, row = rt * NT + r;
+        const float sum = (s_red[r] + s_red[64 + r]) + (s_red[128 + r] + s_red[192 + r]);
+        const bool any = !(sum <= 0.f);
+        s_col[r] = any ? 1.f / sum : 0.f;
+        if (!whole) {
+          a.part_ml[slot * 2 * NT + r] = s_ref[r];
+          a.part_ml[slot * 2 * NT + NT + r] = sum;
+        } else if (row < a.rows) {
+          a.lse[(int64_t)w.b * a.rows + row] = any ? (s_ref[r] + log2f(sum)) * 0.693147180559945309f : -INFINITY;
+        }
+      }
+      named_bar_sync(1, 128);
+      mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.st, 93);
+      tc_fence_after();
+      const int d_c = a.nc * 64;
+      for (int mt = 0; mt < a.nc / 2; mt++)
+        for (int c = 0; c < NT; c += 16) {
+          float o[16];
+          tmem_ld16(tmem + mt * NT + c + lanes, o);
+          tmem_ld_wait();
+          const int d = mt * 128 + warp * 32 + lane;
+          if (!whole) {
+            float* dst = a.part + (slot * NT + c) * d_c + d;
+#pragma unroll
+            for (int i = 0; i < 16; i++) dst[(int64_t)i * d_c] = o[i];
+          } else {
+            // neighbouring lanes trade values, so that each writes two adjacent ones of one row
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float x = o[i] * s_col[c + i], y = o[i + 1] * s_col[c + i + 1];
+              const float z = __shfl_xor_sync(0xffffffffu, lane & 1 ? x : y, 1);
+              const int row = rt * NT + c + i + (lane & 1);
+              const uint32_t two = lane & 1 ? Num<T>::pack(z, y) : Num<T>::pack(x, z);
+              if (row < a.rows)
+                *reinterpret_cast<uint32_t*>(static_cast<T*>(a.out) + ((int64_t)w.b * a.rows + row) * d_c + (d & ~1)) = two;
+            }
+          }
+        }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 5) tmem_dealloc(tmem, 512);
+}
+
+// Joins a split sequence's pieces: out = sum_g 2^(m_g - M) O_g / sum_g 2^(m_g - M) l_g, in CTA order.
+// One block per query row, four values a thread, eight pieces' loads in flight; rows of whole
+// sequences are left alone.
 template <class T>
-__global__ void __launch_bounds__(256) k_paged_simple(const PagedArgs a) {
-  extern __shared__ float sm[];
-  const int D = a.d_c + a.d_r, ld = D + 1;
-  float* qs = sm;                 // [16][D]
-  float* ks = sm + 16 * D;        // [32][ld]
-  const int b = blockIdx.y, warp = threadIdx.x / 32, lane = threadIdx.x % 32, rows = a.Tq * a.H;
-  const int len = min(max(a.lens[b], 0), a.max_pages * a.page_size);
-  for (int i = threadIdx.x; i < 16 * D; i += 256) {
-    const int r = blockIdx.x * 16 + i / D;
-    qs[i] = r < rows ? Num<T>::to_f(static_cast<const T*>(a.q)[b * a.q_b + (r / a.H) * a.q_t + (r % a.H) * a.q_h + i % D]) : 0.f;
-  }
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0, 0}, o[2][16] = {};
-  for (int j0 = 0; j0 < len; j0 += 32) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * D; i += 256) {
-      const int j = j0 + i / D;
-      float v = 0.f;
-      if (j < len) {
-        const int pg = a.bt[b * a.bt_stride + j / a.page_size];
-        if (pg >= 0 && pg < a.pages)
-          v = Num<T>::to_f(static_cast<const T*>(a.cache)[pg * a.page_stride + (j % a.page_size) * a.row_stride + i % D]);
-        else report(a.st, LL_ERR_RANGE, 73, b);
-      }
-      ks[(i / D) * ld + i % D] = v;
+__global__ void __launch_bounds__(128) k_paged_combine(const PagedArgs a, int NT) {
+  const int b = blockIdx.x / a.rows, row = blockIdx.x % a.rows, rt = row / NT, r = row % NT;
+  pdl_wait();
+  const int64_t before = a.starts[b], per = a.starts[a.B];
+  const int64_t last = before + paged_tiles(paged_len(a, b)) - 1;
+  const int g0 = (int)(before / per), g1 = (int)(last / per);
+  if (g0 == g1) return;
+  // a CTA's first piece is in its slot 0, its last (when another) in slot 1
+  auto slot = [&](int g) { return ((int64_t)g * 2 + (before > g * per ? 1 : 0)) * a.RT + rt; };
+  const int d_c = a.nc * 64, d = threadIdx.x * 4, n = g1 - g0 + 1, lane = threadIdx.x % 32;
+  float M = kPgNone;
+  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[slot(g0 + i) * 2 * NT + r]);
+#pragma unroll
+  for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
+  float L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < n; i0 += 8) {
+    float f[8], l[8];
+    float4 x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const int64_t sl = slot(g0 + min(i0 + i, n - 1));
+      f[i] = a.part_ml[sl * 2 * NT + r];
+      l[i] = a.part_ml[sl * 2 * NT + NT + r];
+      x[i] = d < d_c ? *reinterpret_cast<const float4*>(a.part + (sl * NT + r) * d_c + d) : o;
     }
-    __syncthreads();
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const int r = blockIdx.x * 16 + warp * 2 + u;
-      const int lim = len - a.Tq + r / a.H + 1;
-      float s = 0.f;
-      for (int d = 0; d < D; d++) s = fmaf(qs[(warp * 2 + u) * D + d], ks[lane * ld + d], s);
-      s = j0 + lane < lim ? s * a.scale : -INFINITY;
-      float mx = s;
-      for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, off));
-      mx = fmaxf(mx, m[u]);
-      const float ref = mx == -INFINITY ? 0.f : mx;
-      const float p = __expf(s - ref), f = __expf(m[u] - ref);
-      float ps = p;
-      for (int off = 16; off; off >>= 1) ps += __shfl_xor_sync(~0u, ps, off);
-      l[u] = l[u] * f + ps;
-      m[u] = mx;
-      for (int i = 0; i < 16; i++) o[u][i] *= f;
-      for (int j = 0; j < 32; j++) {
-        const float pj = __shfl_sync(~0u, p, j);
-#pragma unroll
-        for (int i = 0; i < 16; i++)
-          if (i * 32 < a.d_c) o[u][i] = fmaf(pj, ks[j * ld + i * 32 + lane], o[u][i]);
-      }
+    for (int i = 0; i < 8; i++) {
+      if (i0 + i >= n) break;
+      const float w = ex2(f[i] - M);
+      L = fmaf(w, l[i], L);
+      o.x = fmaf(w, x[i].x, o.x);
+      o.y = fmaf(w, x[i].y, o.y);
+      o.z = fmaf(w, x[i].z, o.z);
+      o.w = fmaf(w, x[i].w, o.w);
     }
   }
-  for (int u = 0; u < 2; u++) {
-    const int r = blockIdx.x * 16 + warp * 2 + u;
-    if (r >= rows) continue;
-    const int64_t row = (int64_t)b * rows + r;
-    for (int i = 0; i * 32 < a.d_c; i++)
-      static_cast<T*>(a.out)[row * a.d_c + i * 32 + lane] = Num<T>::from_f(l[u] > 0.f ? o[u][i] / l[u] : 0.f);
-    if (lane == 0) a.lse[row] = l[u] > 0.f ? m[u] + logf(l[u]) : -INFINITY;
-  }
+  const bool any = !(L <= 0.f);
+  const float inv = any ? 1.f / L : 0.f;
+  const int64_t at = (int64_t)b * a.rows + row;
+  if (d < d_c)
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * d_c + d) =
+        make_uint2(Num<T>::pack(o.x * inv, o.y * inv), Num<T>::pack(o.z * inv, o.w * inv));
+  if (threadIdx.x == 0) a.lse[at] = any ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+}
+
+// Row tiles of a sequence, their height (a multiple of 16, the tiles' rows nearly equal) and the
+// number of ranges the key tiles are dealt into, so that about every SM has one CTA.
+struct PagedPlan {
+  int RT, NT, G;
+  size_t part, ml;        // workspace floats
+};
+static PagedPlan paged_plan(int Tq, int H, int d_c) {
+  PagedPlan p;
+  const int rows = Tq * H, sms = device_info().sms > 0 ? device_info().sms : 148;
+  p.RT = (rows + 63) / 64;
+  p.NT = ((rows + p.RT - 1) / p.RT + 15) / 16 * 16;
+  p.G = std::max(1, sms / p.RT);
+  p.part = p.G > 1 ? (size_t)p.G * 2 * p.RT * p.NT * d_c : 0;
+  p.ml = p.G > 1 ? (size_t)p.G * 2 * p.RT * 2 * p.NT : 0;
+  return p;
+}
+
+template <class T, int NT>
+static int launch_paged(const PagedTma& tm, const PagedArgs& a, int smem, cudaStream_t s) {
+  LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_paged<T, NT>), smem));
+  return launch_pdl("k_paged", k_paged<T, NT>, dim3(a.G * a.RT), dim3(kPgThreads), smem, s, tm, a);
+}
+
+template <class T>
+static int run_paged(const PagedTma& tm, const PagedArgs& a, int NT, cudaStream_t s) {
+  const int smem = 1024 + 2 * a.nchunk * 8192 + a.nchunk * NT * 128 + kPgKeys * 128 + 128 + 4 * 384;
+  if (NT == 16) LL_TRY((launch_paged<T, 16>(tm, a, smem, s)));
+  else if (NT == 32) LL_TRY((launch_paged<T, 32>(tm, a, smem, s)));
+  else if (NT == 48) LL_TRY((launch_paged<T, 48>(tm, a, smem, s)));
+  else LL_TRY((launch_paged<T, 64>(tm, a, smem, s)));
+  if (a.G == 1) return LL_OK;
+  return launch_pdl("k_paged_combine", k_paged_combine<T>, dim3((unsigned)a.B * a.rows), dim3(128), 0, s, a, NT);
 }
 
 }  // namespace ll
@@ -90,27 +588,71 @@ using namespace ll;
 
 extern "C" {
 
-size_t ll_paged_latent_workspace_bytes(int B, int Tq, int H, int d_c) { return B > 0 && Tq > 0 && H > 0 && d_c > 0 ? 256 : 0; }
+size_t ll_paged_latent_workspace_bytes(int B, int Tq, int H, int d_c) {
+  if (B <= 0 || Tq <= 0 || H <= 0 || d_c <= 0 || (int64_t)Tq * H > (1 << 24)) return 0;
+  const PagedPlan p = paged_plan(Tq, H, d_c);
+  return (p.part + p.ml) * 4 + ((size_t)B + 1) * 8 + 1024;
+}
 
-int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_stride_t, int64_t q_stride_h,
-                              const void* cache, int64_t page_stride, int64_t row_stride, int pages, int page_size,
+int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_stride_row, const void* cache,
+                              int64_t page_stride, int64_t row_stride, int pages, int page_size,
                               const int32_t* block_table, int64_t table_stride, int max_pages, const int32_t* seq_lens,
                               int B, int Tq, int H, int d_c, int d_r, float scale, int dtype, void* out, float* lse,
                               void* workspace, size_t workspace_bytes, void* stream) {
   if (B < 0 || Tq <= 0 || H <= 0 || d_c <= 0 || d_c % 128 || d_c > 512 || (d_r != 0 && d_r != 64) ||
       (dtype != 1 && dtype != 2) || pages <= 0 || page_size <= 0 || page_size % 8 || max_pages <= 0)
     return LL_ERR_ARG;
+  if ((int64_t)Tq * H > (1 << 24) || (int64_t)B * Tq * H > INT32_MAX || (int64_t)max_pages * page_size > INT32_MAX - 64)
+    return LL_ERR_ARG;
   if (B == 0) return LL_OK;
+  const int D = d_c + d_r;
+  if (!q || !cache || !block_table || !seq_lens || !out || !lse || !workspace) return LL_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) |
+       reinterpret_cast<uintptr_t>(workspace)) & 15)
+    return LL_ERR_ARG;
+  if (q_stride_b % 8 || q_stride_row % 8 || q_stride_row < D || q_stride_b < D || page_stride % 8 || row_stride % 8 ||
+      row_stride < D || page_stride < D || table_stride < 0)
+    return LL_ERR_ARG;
+  if (workspace_bytes < ll_paged_latent_workspace_bytes(B, Tq, H, d_c)) return LL_ERR_WORKSPACE;
   LL_TRY(check_arch());
   LL_STREAM(stream);
   g_launch_count = 0;
-  PagedArgs a{q, cache, block_table, seq_lens, out, lse, q_stride_b, q_stride_t, q_stride_h, page_stride, row_stride,
-              table_stride, pages, page_size, max_pages, Tq, H, d_c, d_r, scale, latent_status()};
-  const int D = d_c + d_r, smem = (16 * D + 32 * (D + 1)) * 4;
-  auto kern = dtype == 1 ? k_paged_simple<__nv_bfloat16> : k_paged_simple<__half>;
-  LL_TRY(set_smem_attr(reinterpret_cast<const void*>(kern), smem));
-  kern<<<dim3((Tq * H + 15) / 16, B), 256, smem, s>>>(a);
-  return check_launch("k_paged_simple");
+  const PagedPlan p = paged_plan(Tq, H, d_c);
+  PagedArgs a{};
+  a.bt = block_table;
+  a.lens = seq_lens;
+  a.out = out;
+  a.lse = lse;
+  Carver cv(workspace);
+  a.part = cv.take<float>(p.part);
+  a.part_ml = cv.take<float>(p.ml);
+  a.starts = cv.take<int64_t>((size_t)B + 1);
+  a.bt_stride = table_stride;
+  a.pages = pages;
+  a.page_size = page_size;
+  a.max_pages = max_pages;
+  a.B = B;
+  a.Tq = Tq;
+  a.H = H;
+  a.rows = Tq * H;
+  a.RT = p.RT;
+  a.G = p.G;
+  a.nc = d_c / 64;
+  a.nchunk = D / 64;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.st = latent_status();
+  if (!a.st) return LL_ERR_CUDA;
+  PagedTma tm;
+  const CUtensorMapDataType dt = dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint64_t qd[3] = {(uint64_t)D, (uint64_t)a.rows, (uint64_t)B};
+  const uint64_t qs[2] = {(uint64_t)q_stride_row * 2, (uint64_t)q_stride_b * 2};
+  const uint32_t qb[3] = {64, (uint32_t)p.NT, 1};
+  LL_TRY(make_map_nd(&tm.q, dt, q, 3, qd, qs, qb, CU_TENSOR_MAP_SWIZZLE_128B));
+  const uint64_t kd[4] = {64, (uint64_t)page_size, (uint64_t)a.nchunk, (uint64_t)pages};
+  const uint64_t ks[3] = {(uint64_t)row_stride * 2, 128, (uint64_t)page_stride * 2};
+  const uint32_t kb[4] = {64, 8, (uint32_t)a.nchunk, 1};
+  LL_TRY(make_map_nd(&tm.kv, dt, cache, 4, kd, ks, kb, CU_TENSOR_MAP_SWIZZLE_128B));
+  return dtype == 1 ? run_paged<__nv_bfloat16>(tm, a, p.NT, s) : run_paged<__half>(tm, a, p.NT, s);
 }
 
 }  // extern "C"
