@@ -600,7 +600,7 @@ int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_strid
                               int B, int Tq, int H, int d_c, int d_r, float scale, int dtype, void* out, float* lse,
                               void* workspace, size_t workspace_bytes, void* stream) {
   if (B < 0 || Tq <= 0 || H <= 0 || d_c <= 0 || d_c % 128 || d_c > 512 || (d_r != 0 && d_r != 64) ||
-      (dtype != 1 && dtype != 2) || pages <= 0 || page_size <= 0 || page_size % 8 || max_pages <= 0)
+      (dtype != 1 && dtype != 2) || pages <= 0 || page_size <= 0 || page_size % 8 || max_pages <= 0 || !(scale > 0.f))
     return LL_ERR_ARG;
   if ((int64_t)Tq * H > (1 << 24) || (int64_t)B * Tq * H > INT32_MAX || (int64_t)max_pages * page_size > INT32_MAX - 64)
     return LL_ERR_ARG;
