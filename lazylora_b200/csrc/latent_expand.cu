@@ -3,174 +3,10 @@
 //   s_ij = scale q_i . k_j (visible j),  p = softmax(s),  o_i = sum_j p_ij v_j,
 //   dv_j = sum_i p_ij g_i,  dp_ij = g_i . v_j,  ds_ij = p_ij (dp_ij - g_i . o_i) scale,
 //   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i;  dk_pe sums dk's rotary part over the heads.
-// First form: one block per (32 rows, head), each warp four rows, a lane per row of the other side;
-// CUDA cores throughout. The backward pass runs one kernel over query rows (dq) and one over key
-// rows (dk, dv), so that every sum has a fixed order.
+// Tiles are dealt from the cumulative lengths on the device; nothing is read back.
 #include "latent_ops.cuh"
 
 namespace ll {
-
-struct ExpandArgs {
-  ll_latent_packed p;
-  const void* g;
-  int64_t g_t, g_h;
-  const void* o;
-  const float* lse_in;
-  void* out;
-  float* lse;
-  void *dq, *dk, *dkpe, *dv;
-  float* dkpe_ws;          // [H][Tk][d_r]
-};
-
-template <class T>
-LL_DEV float k_at(const ll_latent_packed& p, int64_t row, int h, int d) {
-  return Num<T>::to_f(d < p.d_n ? static_cast<const T*>(p.k_nope)[row * p.k_stride_t + h * p.k_stride_h + d]
-                                : static_cast<const T*>(p.k_pe)[row * p.kpe_stride_t + d - p.d_n]);
-}
-template <class T>
-LL_DEV float q_at(const ll_latent_packed& p, int64_t row, int h, int d) {
-  return Num<T>::to_f(static_cast<const T*>(p.q)[row * p.q_stride_t + h * p.q_stride_h + d]);
-}
-template <class T>
-LL_DEV float v_at(const ll_latent_packed& p, int64_t row, int h, int d) {
-  return Num<T>::to_f(static_cast<const T*>(p.v)[row * p.v_stride_t + h * p.v_stride_h + d]);
-}
-template <class T>
-LL_DEV float g_at(const ExpandArgs& a, int64_t row, int h, int d) {
-  return Num<T>::to_f(static_cast<const T*>(a.g)[row * a.g_t + h * a.g_h + d]);
-}
-
-constexpr int kDk = 192, kDv = 128;
-
-// MODE 0: forward; 1: dq; 2: dk and dv (rows are keys, the other side queries).
-template <class T, int MODE>
-__global__ void __launch_bounds__(256) k_expand_simple(const ExpandArgs a) {
-  extern __shared__ float sm[];
-  const ll_latent_packed& p = a.p;
-  float* rk = sm;                        // own rows [32][192]: q, or k
-  float* rv = rk + 32 * kDk;             // own rows [32][128]: g, or v
-  float* ck = rv + 32 * kDv;             // other side [32][193]: k, or q
-  float* cv = ck + 32 * (kDk + 1);       // other side [32][129]: v, or g
-  float* cl = cv + 32 * (kDv + 1);       // lse and delta of the other side (MODE 2)
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, h = blockIdx.y;
-  const int DK = p.d_n + p.d_r, DV = p.d_v;
-  int b, r0;
-  if (!find_tile_from_end(MODE == 2 ? p.cu_k : p.cu_q, p.B, MODE == 2 ? p.Tk : p.Tq, 32, blockIdx.x, b, r0)) return;
-  int q_lo, q_hi, k_lo, k_hi;
-  seq_range(p.cu_q, b, p.Tq, q_lo, q_hi);
-  seq_range(p.cu_k, b, p.Tk, k_lo, k_hi);
-  const int nq = q_hi - q_lo, nk = k_hi - k_lo, shift = nk - nq;
-  const int n_row = MODE == 2 ? nk : nq, n_col = MODE == 2 ? nq : nk;
-  const int64_t row_base = MODE == 2 ? k_lo : q_lo, col_base = MODE == 2 ? q_lo : k_lo;
-  for (int i = threadIdx.x; i < 32 * DK; i += 256) {
-    const int r = r0 + i / DK, d = i % DK;
-    rk[(i / DK) * kDk + d] = r < n_row ? (MODE == 2 ? k_at<T>(p, row_base + r, h, d) : q_at<T>(p, row_base + r, h, d)) : 0.f;
-  }
-  if (MODE != 0)
-    for (int i = threadIdx.x; i < 32 * DV; i += 256) {
-      const int r = r0 + i / DV, d = i % DV;
-      rv[(i / DV) * kDv + d] = r < n_row ? (MODE == 2 ? v_at<T>(p, row_base + r, h, d) : g_at<T>(a, row_base + r, h, d)) : 0.f;
-    }
-  __syncthreads();
-  float m[4], l[4] = {}, x[4][6] = {}, y[4][4] = {}, rl[4], rd[4];
-  for (int u = 0; u < 4; u++) {
-    m[u] = -INFINITY;
-    if (MODE == 1) {
-      const int r = r0 + warp * 4 + u;
-      float d = 0.f;
-      if (r < n_row)
-        for (int i = lane; i < DV; i += 32)
-          d += rv[(warp * 4 + u) * kDv + i] * Num<T>::to_f(static_cast<const T*>(a.o)[((row_base + r) * p.H + h) * DV + i]);
-      for (int off = 16; off; off >>= 1) d += __shfl_xor_sync(~0u, d, off);
-      rd[u] = d;
-      rl[u] = r < n_row ? a.lse_in[(int64_t)h * p.Tq + row_base + r] : 0.f;
-    }
-  }
-  for (int c0 = 0; c0 < n_col; c0 += 32) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < 32 * DK; i += 256) {
-      const int c = c0 + i / DK, d = i % DK;
-      ck[(i / DK) * (kDk + 1) + d] = c < n_col ? (MODE == 2 ? q_at<T>(p, col_base + c, h, d) : k_at<T>(p, col_base + c, h, d)) : 0.f;
-    }
-    for (int i = threadIdx.x; i < 32 * DV; i += 256) {
-      const int c = c0 + i / DV, d = i % DV;
-      cv[(i / DV) * (kDv + 1) + d] = c < n_col ? (MODE == 2 ? g_at<T>(a, col_base + c, h, d) : v_at<T>(p, col_base + c, h, d)) : 0.f;
-    }
-    __syncthreads();
-    if (MODE == 2) {
-      if (threadIdx.x < 32) {
-        const int c = c0 + lane;
-        float d = 0.f;
-        if (c < n_col)
-          for (int i = 0; i < DV; i++)
-            d += cv[lane * (kDv + 1) + i] * Num<T>::to_f(static_cast<const T*>(a.o)[((col_base + c) * p.H + h) * DV + i]);
-        cl[lane] = c < n_col ? a.lse_in[(int64_t)h * p.Tq + col_base + c] : 0.f;
-        cl[32 + lane] = d;
-      }
-      __syncthreads();
-    }
-    for (int u = 0; u < 4; u++) {
-      const int r = r0 + warp * 4 + u, c = c0 + lane;
-      const int qi = MODE == 2 ? c : r, ki = MODE == 2 ? r : c;
-      const bool seen = qi < nq && ki < nk && (!p.causal || ki <= qi + shift);
-      float s = 0.f, dp = 0.f;
-      for (int d = 0; d < DK; d++) s = fmaf(rk[(warp * 4 + u) * kDk + d], ck[lane * (kDk + 1) + d], s);
-      s = seen ? s * p.scale : -INFINITY;
-      if (MODE == 0) {
-        float mx = s;
-        for (int off = 16; off; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, off));
-        mx = fmaxf(mx, m[u]);
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        const float pr = __expf(s - ref), f = __expf(m[u] - ref);
-        float ps = pr;
-        for (int off = 16; off; off >>= 1) ps += __shfl_xor_sync(~0u, ps, off);
-        l[u] = l[u] * f + ps;
-        m[u] = mx;
-        for (int i = 0; i < 4; i++) y[u][i] *= f;
-        for (int j = 0; j < 32; j++) {
-          const float pj = __shfl_sync(~0u, pr, j);
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (i * 32 < DV) y[u][i] = fmaf(pj, cv[j * (kDv + 1) + i * 32 + lane], y[u][i]);
-        }
-      } else {
-        for (int d = 0; d < DV; d++) dp = fmaf(rv[(warp * 4 + u) * kDv + d], cv[lane * (kDv + 1) + d], dp);
-        const float lse = MODE == 1 ? rl[u] : cl[lane], delta = MODE == 1 ? rd[u] : cl[32 + lane];
-        const float pr = seen ? __expf(s - lse) : 0.f;
-        const float ds = seen ? pr * (dp - delta) * p.scale : 0.f;
-        for (int j = 0; j < 32; j++) {
-          const float dj = __shfl_sync(~0u, ds, j), pj = __shfl_sync(~0u, pr, j);
-#pragma unroll
-          for (int i = 0; i < 6; i++)
-            if (i * 32 < DK) x[u][i] = fmaf(dj, ck[j * (kDk + 1) + i * 32 + lane], x[u][i]);
-          if (MODE == 2)
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (i * 32 < DV) y[u][i] = fmaf(pj, cv[j * (kDv + 1) + i * 32 + lane], y[u][i]);
-        }
-      }
-    }
-  }
-  for (int u = 0; u < 4; u++) {
-    const int r = r0 + warp * 4 + u;
-    if (r >= n_row) continue;
-    const int64_t row = row_base + r;
-    if (MODE == 0) {
-      for (int i = 0; i * 32 < DV; i++)
-        static_cast<T*>(a.out)[(row * p.H + h) * DV + i * 32 + lane] = Num<T>::from_f(l[u] > 0.f ? y[u][i] / l[u] : 0.f);
-      if (lane == 0) a.lse[(int64_t)h * p.Tq + row] = l[u] > 0.f ? m[u] + logf(l[u]) : -INFINITY;
-    } else if (MODE == 1) {
-      for (int i = 0; i * 32 < DK; i++) static_cast<T*>(a.dq)[(row * p.H + h) * DK + i * 32 + lane] = Num<T>::from_f(x[u][i]);
-    } else {
-      for (int i = 0; i * 32 < DV; i++) static_cast<T*>(a.dv)[(row * p.H + h) * DV + i * 32 + lane] = Num<T>::from_f(y[u][i]);
-      for (int i = 0; i * 32 < DK; i++) {
-        const int d = i * 32 + lane;
-        if (d < p.d_n) static_cast<T*>(a.dk)[(row * p.H + h) * p.d_n + d] = Num<T>::from_f(x[u][i]);
-        else a.dkpe_ws[((int64_t)h * p.Tk + row) * p.d_r + d - p.d_n] = x[u][i];
-      }
-    }
-  }
-}
 
 // ------------------------------------------------------------------------------- forward
 // One CTA takes 256 query rows of one sequence and head as two tiles of 128 that alternate: while one
@@ -299,7 +135,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
   __syncwarp();
   pdl_wait();
   int b, q0, q_lo, q_hi, k_lo, k_hi;
-  const bool any = find_tile_from_end(a.cu_q, a.B, a.Tq, 256, blockIdx.x, b, q0);
+  const bool any = find_tile<true>(a.cu_q, a.B, a.Tq, 256, blockIdx.x, b, q0);
   if (any) {
     seq_range(a.cu_q, b, a.Tq, q_lo, q_hi);
     seq_range(a.cu_k, b, a.Tk, k_lo, k_hi);
@@ -537,14 +373,525 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
   if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-// dk_pe[row][d] = sum over heads, heads in order.
+// ------------------------------------------------------------------------------- backward
+// Two kernels, one over query rows (dq) and one over key rows (dk, dv): each output row is summed by one
+// CTA in a fixed order, at the price of computing S and dP twice (7 products for 5). Both keep the tensor
+// cores one step ahead of the element-wise work, which turns S and dP into P and dS:
+//   issue order  S(i + 1), dP(i + 1), then the sums over step i.
+// P and dS reach the tensor cores through tensor memory, rounded to the 16-bit type (as the gradients
+// themselves); scale is applied to the fp32 sums. Per step the products take 2048 (dq: 128 keys) and
+// about 1400 cycles (dk, dv: 64 queries) against 1024 and 512 of exponentials.
+//
+// Tensor memory, 512 columns each:
+//   dq:     S 0 (128), dP 128 (128), dQ 256 (192), dS 448 (64)
+//   dk, dv: S^T 0 (64), dP^T 64 (64), dV 128 (128), dK 256 (192), P^T 448 (32), dS^T 480 (32)
+// Threads: warps 0-3 and 4-7 the element-wise work, each group half of a tile's columns; 8 TMA; 9 MMA; 10
+// (dk, dv) the queries' statistics.
+struct ExBwdArgs {
+  const int32_t *cu_q, *cu_k;
+  const void *g, *o;
+  int64_t g_t, g_h;
+  const float* lse;
+  float* delta;            // [H][Tq]: written by the dq kernel, read by the other
+  float* dkpe;             // [H][Tk][64 nr]
+  void *dq, *dk, *dv;
+  int B, Tq, Tk, H, nn, nr, nv, causal;
+  float scale, scale_log2;
+  DevStatus* st;
+};
+
+// 32 columns of an accumulator, times f, as 32 values of the 16-bit type.
 template <class T>
-__global__ void k_sum_heads(const float* __restrict__ ws, int H, int64_t n, T* __restrict__ out) {
-  const int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x;
+LL_DEV void store32(T* dst, const uint32_t* o, float f) {
+#pragma unroll
+  for (int k = 0; k < 32; k += 8) {
+    uint32_t w[4];
+#pragma unroll
+    for (int z = 0; z < 4; z++) w[z] = Num<T>::pack(__uint_as_float(o[k + 2 * z]) * f, __uint_as_float(o[k + 2 * z + 1]) * f);
+    *reinterpret_cast<uint4*>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+LL_DEV void load_acc32(uint32_t at, uint32_t* o, bool any) {
+  if (any) {
+    ld32(at, o);
+    tmem_ld_wait();
+    ld32_ready(o);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 32; k++) o[k] = 0;
+  }
+}
+// Rows from .. rows - 1 of `chunks` consecutive chunks of `rows` rows to zero, by 256 threads.
+LL_DEV void zero_tail(uint8_t* at, int chunks, int rows, int from) {
+  for (int i = threadIdx.x; i < (rows - from) * chunks * 8; i += 256) {
+    const int c = i / ((rows - from) * 8), j = i % ((rows - from) * 8);
+    *reinterpret_cast<uint4*>(at + (c * rows + from) * 128 + j * 16) = make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <class T>
+__global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__ ExTma tm, const ExBwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nqk = a.nn + a.nr;
+  uint8_t* s_q = base;
+  uint8_t* s_g = s_q + nqk * kExChunk;
+  uint8_t* s_k = s_g + a.nv * kExChunk;                   // two key tiles
+  uint8_t* s_v = s_k + 2 * nqk * kExChunk;                // one value tile
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + a.nv * kExChunk);
+  uint64_t *q_full = bars, *k_full = bars + 1, *k_rel = bars + 3, *v_full = bars + 5, *v_rel = bars + 6,
+           *sp_full = bars + 7, *sp_free = bars + 8, *ds_ready = bars + 9, *acc_done = bars + 10, *drain = bars + 11;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 12; i++) mbar_init(&bars[i], i == 8 || i == 9 ? 8 : 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tm.q);
+    tma_prefetch_desc(&tm.g);
+    tma_prefetch_desc(&tm.kn);
+    tma_prefetch_desc(&tm.kp);
+    tma_prefetch_desc(&tm.v);
+  }
+  __syncwarp();
+  pdl_wait();
+  int b, q0, q_lo = 0, q_hi = 0, k_lo = 0, k_hi = 0;
+  if (find_tile<true>(a.cu_q, a.B, a.Tq, 128, blockIdx.x, b, q0)) {
+    seq_range(a.cu_q, b, a.Tq, q_lo, q_hi);
+    seq_range(a.cu_k, b, a.Tk, k_lo, k_hi);
+  } else {
+    q0 = 0;
+  }
+  const int nq = q_hi - q_lo, nk = k_hi - k_lo, n = key_tiles(q0, 128, nq, nk, a.causal);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_next();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
+    if (warp == 8 && lane == 0 && n > 0) {
+      // ----------------------------------------------------------------------------- TMA
+      bool ok = true;
+      mbar_arrive_expect_tx(q_full, (nqk + a.nv) * kExChunk);
+      for (int c = 0; c < nqk; c++) tma_load_3d(s_q + c * kExChunk, &tm.q, q_full, c * 64, head, q_lo + q0);
+      for (int c = 0; c < a.nv; c++) tma_load_3d(s_g + c * kExChunk, &tm.g, q_full, c * 64, head, q_lo + q0);
+      int nk_loads = 0, nv_loads = 0;
+      for (int i = 0; i < n && ok; i++) {
+        if (!(ok = mbar_wait(&k_rel[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.st, 121))) break;
+        mbar_arrive_expect_tx(&k_full[i & 1], nqk * kExChunk);
+        for (int c = 0; c < nqk; c++) {
+          uint8_t* dst = s_k + ((i & 1) * nqk + c) * kExChunk;
+          if (c < a.nn) tma_load_3d(dst, &tm.kn, &k_full[i & 1], c * 64, head, k_lo + i * 128);
+          else tma_load_2d(dst, &tm.kp, &k_full[i & 1], (c - a.nn) * 64, k_lo + i * 128);
+        }
+        nk_loads++;
+        if (!(ok = mbar_wait(v_rel, (i & 1) ^ 1, abort_flag, a.st, 122))) break;
+        mbar_arrive_expect_tx(v_full, a.nv * kExChunk);
+        for (int c = 0; c < a.nv; c++) tma_load_3d(s_v + c * kExChunk, &tm.v, v_full, c * 64, head, k_lo + i * 128);
+        nv_loads++;
+      }
+      volatile int keep = 0;                   // everything issued has landed, also after an abort
+      mbar_wait_sleep(q_full, 0, &keep, a.st, 123, 64);
+      for (int i = max(0, nk_loads - 2); i < nk_loads; i++) mbar_wait_sleep(&k_full[i & 1], (i >> 1) & 1, &keep, a.st, 124, 64);
+      if (nv_loads > 0) mbar_wait_sleep(v_full, (nv_loads - 1) & 1, &keep, a.st, 125, 64);
+    }
+    __syncwarp();
+    if (warp == 9) {
+      // ----------------------------------------------------------------------------- MMA
+      const bool lead = elect_one();
+      const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, 128, false, false);
+      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, 64, false, true);
+      const MmaDesc q_d(smem_u32(s_q), 16, 1024), g_d(smem_u32(s_g), 16, 1024), k_d(smem_u32(s_k), 16, 1024),
+          v_d(smem_u32(s_v), 16, 1024), kt_d(smem_u32(s_k), 1024, 1024);
+      const uint32_t k_tile = nqk * (kExChunk / 16);
+      bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag, a.st, 126);
+#pragma unroll 1
+      for (int i = -1; i < n && ok; i++) {
+        if (i >= 0 && !(ok = mbar_wait(sp_free, i & 1, abort_flag, a.st, 127))) break;
+        const int j = i + 1;
+        if (j < n) {
+          if (!(ok = mbar_wait(&k_full[j & 1], (j >> 1) & 1, abort_flag, a.st, 128))) break;
+          tc_fence_after();
+          if (lead) {
+#pragma unroll 1
+            for (int c = 0; c < nqk; c++)
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                mma_16bit(tmem, q_d.lo + c * (kExChunk / 16) + kk * 2, q_d.hi,
+                          k_d.lo + (j & 1) * k_tile + c * (kExChunk / 16) + kk * 2, k_d.hi, id_s, c + kk);
+          }
+          if (!(ok = mbar_wait(v_full, j & 1, abort_flag, a.st, 129))) break;
+          tc_fence_after();
+          if (lead) {
+#pragma unroll 1
+            for (int c = 0; c < a.nv; c++)
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                mma_16bit(tmem + 128, g_d.lo + c * (kExChunk / 16) + kk * 2, g_d.hi, v_d.lo + c * (kExChunk / 16) + kk * 2,
+                          v_d.hi, id_s, c + kk);
+            mma_commit(sp_full);
+            mma_commit(v_rel);
+          }
+        }
+        if (i < 0) continue;
+        if (!(ok = mbar_wait(ds_ready, i & 1, abort_flag, a.st, 130))) break;
+        tc_fence_after();
+        if (lead) {
+#pragma unroll 1
+          for (int c = 0; c < nqk; c++)
+#pragma unroll
+            for (int kk = 0; kk < 8; kk++)
+              mma_16bit_ts(tmem + 256 + c * 64, tmem + 448 + kk * 8,
+                           kt_d.lo + (i & 1) * k_tile + c * (kExChunk / 16) + kk * 128, kt_d.hi, id_o, i + kk);
+          mma_commit(&k_rel[i & 1]);
+          mma_commit(acc_done);
+        }
+      }
+      if (lead) mma_commit(drain);
+      volatile int keep = 0;
+      mbar_wait_sleep(drain, 0, &keep, a.st, 131, 64);
+      __syncwarp();
+    }
+  } else {
+    // ---------------------------------------------------------------------- element-wise
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExRegsMore));
+    const int cw = warp / 4;
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    const int row = q0 + (warp % 4) * 32 + lane;
+    const int see = a.causal ? min(nk, row + nk - nq + 1) : nk, see_all = a.causal ? min(nk, q0 + nk - nq + 1) : nk;
+    float delta = 0.f, lse2 = 0.f;
+    if (row < nq) {
+      const uint4* gp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.g) + (q_lo + row) * a.g_t + head * a.g_h);
+      const uint4* op = reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + ((int64_t)(q_lo + row) * a.H + head) * (a.nv * 64));
+      for (int i = 0; i < a.nv * 8; i++) {
+        const uint4 gv = gp[i], ov = op[i];
+        const T *gx = reinterpret_cast<const T*>(&gv), *ox = reinterpret_cast<const T*>(&ov);
+#pragma unroll
+        for (int z = 0; z < 8; z++) delta = fmaf(Num<T>::to_f(gx[z]), Num<T>::to_f(ox[z]), delta);
+      }
+      const int64_t at = (int64_t)head * a.Tq + q_lo + row;
+      lse2 = a.lse[at] * 1.4426950408889634f;
+      if (cw == 0) a.delta[at] = delta;
+    }
+    bool ok = true;
+    for (int i = 0; i < n; i++) {
+      if (!(ok = mbar_wait(sp_full, i & 1, abort_flag, a.st, 132))) break;
+      tc_fence_after();
+      uint32_t x[64], y[64];
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        ld32(tmem + lanes + cw * 64 + c, x + c);
+        ld32(tmem + 128 + lanes + cw * 64 + c, y + c);
+      }
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 64; c += 32) {
+        ld32_ready(x + c);
+        ld32_ready(y + c);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sp_free);
+      if (i * 128 + 128 > nk) {                // key rows past the end must not meet dS's zeros
+        zero_tail(s_k + (i & 1) * nqk * kExChunk, nqk, 128, nk - i * 128);
+        fence_async_smem();
+      }
+      const bool part = i * 128 + 128 > see_all;
+      const int lim = see - i * 128 - cw * 64;
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 64; c += 2) {
+        float d[2];
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+          const float p = ex2(fmaf(__uint_as_float(x[c + z]), a.scale_log2, -lse2));
+          d[z] = p * (__uint_as_float(y[c + z]) - delta);
+          if (part && c + z >= lim) d[z] = 0.f;
+        }
+        w[c / 2] = Num<T>::pack(d[0], d[1]);
+      }
+      if (i > 0 && !(ok = mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 133))) break;
+      tc_fence_after();
+      st32(tmem + 448 + lanes + cw * 32, w);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 134);
+    tc_fence_after();
+    T* dst = static_cast<T*>(a.dq) + ((int64_t)(q_lo + row) * a.H + head) * (nqk * 64);
+    for (int c = cw * 32; c < nqk * 64; c += 64) {
+      uint32_t o[32];
+      load_acc32(tmem + 256 + lanes + c, o, n > 0);
+      if (row < nq) store32<T>(dst + c, o, a.scale);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+constexpr int kExQ = 64;                 // query rows a step of the key-row kernel
+constexpr int kExQStages = 3;
+constexpr int kExQChunk = kExQ * 128;    // bytes
+
+template <class T>
+__global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant__ ExTma tm, const ExBwdArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int nqk = a.nn + a.nr, stage = (nqk + a.nv) * kExQChunk;
+  uint8_t* s_k = base;
+  uint8_t* s_v = s_k + nqk * kExChunk;
+  uint8_t* s_qg = s_v + a.nv * kExChunk;                  // stages of Q and dO
+  float4* s_stat = reinterpret_cast<float4*>(s_qg + kExQStages * stage);      // [stage][32]: (lse, delta) of two queries
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_stat + kExQStages * 32);
+  uint64_t *kv_full = bars, *q_full = bars + 1, *q_rel = q_full + kExQStages, *st_full = q_rel + kExQStages,
+           *sp_full = st_full + kExQStages, *sp_free = sp_full + 1, *ds_ready = sp_full + 2, *acc_done = sp_full + 3,
+           *drain = sp_full + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 3 * kExQStages + 6; i++) mbar_init(&bars[i], &bars[i] == sp_free || &bars[i] == ds_ready ? 8 : 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == 8 && lane == 0) {
+    tma_prefetch_desc(&tm.q);
+    tma_prefetch_desc(&tm.g);
+    tma_prefetch_desc(&tm.kn);
+    tma_prefetch_desc(&tm.kp);
+    tma_prefetch_desc(&tm.v);
+  }
+  __syncwarp();
+  pdl_wait();
+  int b, k0, q_lo = 0, q_hi = 0, k_lo = 0, k_hi = 0;
+  if (find_tile<false>(a.cu_k, a.B, a.Tk, 128, blockIdx.x, b, k0)) {
+    seq_range(a.cu_q, b, a.Tq, q_lo, q_hi);
+    seq_range(a.cu_k, b, a.Tk, k_lo, k_hi);
+  } else {
+    k0 = 0;
+  }
+  const int nq = q_hi - q_lo, nk = k_hi - k_lo, shift = nk - nq;
+  // the queries from the first that sees key k0 on
+  const int first = k0 >= nk ? nq : a.causal ? max(0, k0 - shift) / kExQ * kExQ : 0;
+  const int n = first < nq ? (nq - first + kExQ - 1) / kExQ : 0;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_next();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
+    if (warp == 8 && lane == 0 && n > 0) {
+      // ----------------------------------------------------------------------------- TMA
+      mbar_arrive_expect_tx(kv_full, (nqk + a.nv) * kExChunk);
+      for (int c = 0; c < nqk; c++) {
+        if (c < a.nn) tma_load_3d(s_k + c * kExChunk, &tm.kn, kv_full, c * 64, head, k_lo + k0);
+        else tma_load_2d(s_k + c * kExChunk, &tm.kp, kv_full, (c - a.nn) * 64, k_lo + k0);
+      }
+      for (int c = 0; c < a.nv; c++) tma_load_3d(s_v + c * kExChunk, &tm.v, kv_full, c * 64, head, k_lo + k0);
+      int i = 0;
+      for (; i < n; i++) {
+        const int s = i % kExQStages;
+        if (!mbar_wait(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 141)) break;
+        mbar_arrive_expect_tx(&q_full[s], stage);
+        const int row = q_lo + first + i * kExQ;
+        for (int c = 0; c < nqk; c++) tma_load_3d(s_qg + s * stage + c * kExQChunk, &tm.q, &q_full[s], c * 64, head, row);
+        for (int c = 0; c < a.nv; c++)
+          tma_load_3d(s_qg + s * stage + (nqk + c) * kExQChunk, &tm.g, &q_full[s], c * 64, head, row);
+      }
+      volatile int keep = 0;                   // everything issued has landed, also after an abort
+      mbar_wait_sleep(kv_full, 0, &keep, a.st, 142, 64);
+      for (int k = max(0, i - kExQStages); k < i; k++)
+        mbar_wait_sleep(&q_full[k % kExQStages], (k / kExQStages) & 1, &keep, a.st, 143, 64);
+    }
+    __syncwarp();
+    if (warp == 9) {
+      // ----------------------------------------------------------------------------- MMA
+      const bool lead = elect_one();
+      const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, kExQ, false, false);
+      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, 64, false, true);
+      const MmaDesc k_d(smem_u32(s_k), 16, 1024), v_d(smem_u32(s_v), 16, 1024), q_d(smem_u32(s_qg), 16, 1024),
+          qt_d(smem_u32(s_qg), 1024, 1024);
+      constexpr uint32_t QC = kExQChunk / 16;
+      const uint32_t stage16 = stage / 16;
+      bool ok = n == 0 || mbar_wait(kv_full, 0, abort_flag, a.st, 144);
+#pragma unroll 1
+      for (int i = -1; i < n && ok; i++) {
+        if (i >= 0 && !(ok = mbar_wait(sp_free, i & 1, abort_flag, a.st, 145))) break;
+        const int j = i + 1;
+        if (j < n) {
+          const int s = j % kExQStages;
+          if (!(ok = mbar_wait(&q_full[s], (j / kExQStages) & 1, abort_flag, a.st, 146))) break;
+          tc_fence_after();
+          if (lead) {
+            const uint32_t at = q_d.lo + s * stage16;
+#pragma unroll 1
+            for (int c = 0; c < nqk; c++)
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                mma_16bit(tmem, k_d.lo + c * (kExChunk / 16) + kk * 2, k_d.hi, at + c * QC + kk * 2, q_d.hi, id_s, c + kk);
+#pragma unroll 1
+            for (int c = 0; c < a.nv; c++)
+#pragma unroll
+              for (int kk = 0; kk < 4; kk++)
+                mma_16bit(tmem + 64, v_d.lo + c * (kExChunk / 16) + kk * 2, v_d.hi, at + (nqk + c) * QC + kk * 2, q_d.hi,
+                          id_s, c + kk);
+            mma_commit(sp_full);
+          }
+        }
+        if (i < 0) continue;
+        if (!(ok = mbar_wait(ds_ready, i & 1, abort_flag, a.st, 147))) break;
+        tc_fence_after();
+        if (lead) {
+          const uint32_t at = qt_d.lo + (i % kExQStages) * stage16;
+#pragma unroll 1
+          for (int c = 0; c < a.nv; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit_ts(tmem + 128 + c * 64, tmem + 448 + kk * 8, at + (nqk + c) * QC + kk * 128, qt_d.hi, id_o, i + kk);
+#pragma unroll 1
+          for (int c = 0; c < nqk; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit_ts(tmem + 256 + c * 64, tmem + 480 + kk * 8, at + c * QC + kk * 128, qt_d.hi, id_o, i + kk);
+          mma_commit(&q_rel[i % kExQStages]);
+          mma_commit(acc_done);
+        }
+      }
+      if (lead) mma_commit(drain);
+      volatile int keep = 0;
+      mbar_wait_sleep(drain, 0, &keep, a.st, 148, 64);
+      __syncwarp();
+    } else if (warp == 10) {
+      // ------------------------------------------------- statistics of the steps' queries
+      for (int i = 0; i < n; i++) {
+        const int s = i % kExQStages;
+        if (!mbar_wait(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 149)) break;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+          const int q = first + i * kExQ + lane * 2 + z;
+          if (q < nq) {
+            const int64_t at = (int64_t)head * a.Tq + q_lo + q;
+            v[2 * z] = a.lse[at] * 1.4426950408889634f;
+            v[2 * z + 1] = a.delta[at];
+          }
+        }
+        s_stat[s * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&st_full[s]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------------- element-wise
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExRegsMore));
+    const int cw = warp / 4;
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    const int row = k0 + (warp % 4) * 32 + lane;
+    bool ok = true;
+    for (int i = 0; i < n; i++) {
+      const int s = i % kExQStages, qa = first + i * kExQ;
+      if (!(ok = mbar_wait(&st_full[s], (i / kExQStages) & 1, abort_flag, a.st, 150))) break;
+      if (!(ok = mbar_wait(sp_full, i & 1, abort_flag, a.st, 151))) break;
+      tc_fence_after();
+      uint32_t x[32], y[32];
+      ld32(tmem + lanes + cw * 32, x);
+      ld32(tmem + 64 + lanes + cw * 32, y);
+      tmem_ld_wait();
+      ld32_ready(x);
+      ld32_ready(y);
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sp_free);
+      if (qa + kExQ > nq) {                    // query rows past the end must not meet zeros of P and dS
+        zero_tail(s_qg + s * stage, nqk + a.nv, kExQ, nq - qa);
+        fence_async_smem();
+      }
+      const bool part = qa + kExQ > nq || (a.causal && k0 + 127 > qa + shift);
+      const int from = (a.causal ? row - shift - qa : 0) - cw * 32, to = nq - qa - cw * 32;   // queries that see the row
+      uint32_t pw[16], dw[16];
+#pragma unroll
+      for (int c = 0; c < 32; c += 2) {
+        const float4 sd = s_stat[s * 32 + cw * 16 + c / 2];
+        float p[2], d[2];
+#pragma unroll
+        for (int z = 0; z < 2; z++) {
+          p[z] = ex2(fmaf(__uint_as_float(x[c + z]), a.scale_log2, -(z ? sd.z : sd.x)));
+          d[z] = p[z] * (__uint_as_float(y[c + z]) - (z ? sd.w : sd.y));
+          if (part && (c + z < from || c + z >= to)) p[z] = d[z] = 0.f;
+        }
+        pw[c / 2] = Num<T>::pack(p[0], p[1]);
+        dw[c / 2] = Num<T>::pack(d[0], d[1]);
+      }
+      if (i > 0 && !(ok = mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 152))) break;
+      tc_fence_after();
+      tmem_st16(tmem + 448 + lanes + cw * 16, pw);
+      tmem_st16(tmem + 480 + lanes + cw * 16, dw);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_ready);
+    }
+    if (ok && n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 153);
+    tc_fence_after();
+    const int64_t at = (int64_t)(k_lo + row) * a.H + head;
+    for (int c = cw * 32; c < a.nv * 64; c += 64) {
+      uint32_t o[32];
+      load_acc32(tmem + 128 + lanes + c, o, n > 0);
+      if (row < nk) store32<T>(static_cast<T*>(a.dv) + at * (a.nv * 64) + c, o, 1.f);
+    }
+    for (int c = cw * 32; c < nqk * 64; c += 64) {
+      uint32_t o[32];
+      load_acc32(tmem + 256 + lanes + c, o, n > 0);
+      if (row >= nk) continue;
+      if (c < a.nn * 64) {
+        store32<T>(static_cast<T*>(a.dk) + at * (a.nn * 64) + c, o, a.scale);
+      } else {
+        float* dst = a.dkpe + ((int64_t)head * a.Tk + k_lo + row) * (a.nr * 64) + c - a.nn * 64;
+#pragma unroll
+        for (int k = 0; k < 32; k += 4)
+          *reinterpret_cast<float4*>(dst + k) =
+              make_float4(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale,
+                          __uint_as_float(o[k + 2]) * a.scale, __uint_as_float(o[k + 3]) * a.scale);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+// dk_pe[row][d] = sum over the heads, in their order; four values a thread, eight heads' loads in flight.
+template <class T>
+__global__ void __launch_bounds__(256) k_ex_sum_heads(const float* __restrict__ ws, int H, int64_t n, T* __restrict__ out) {
+  pdl_wait();
+  const int64_t i = (blockIdx.x * (int64_t)blockDim.x + threadIdx.x) * 4;
   if (i >= n) return;
-  float s = 0.f;
-  for (int h = 0; h < H; h++) s += ws[h * n + i];
-  out[i] = Num<T>::from_f(s);
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int h0 = 0; h0 < H; h0 += 8) {
+    float4 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] = *reinterpret_cast<const float4*>(ws + (int64_t)min(h0 + k, H - 1) * n + i);
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+      if (h0 + k < H) { s.x += v[k].x; s.y += v[k].y; s.z += v[k].z; s.w += v[k].w; }
+  }
+  *reinterpret_cast<uint2*>(out + i) = make_uint2(Num<T>::pack(s.x, s.y), Num<T>::pack(s.z, s.w));
 }
 
 // A 16-byte aligned pointer with positive strides that are multiples of 16 bytes, as the tensor maps take.
@@ -594,13 +941,29 @@ static int check_packed(const ll_latent_packed* p) {
   return LL_OK;
 }
 
-template <class T, int MODE>
-static int launch_simple(const ExpandArgs& a, cudaStream_t s) {
-  const int smem = (32 * kDk + 32 * kDv + 32 * (kDk + 1) + 32 * (kDv + 1) + 64) * 4;
-  LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_expand_simple<T, MODE>), smem));
-  const int tiles = (MODE == 2 ? a.p.Tk : a.p.Tq) / 32 + a.p.B;
-  k_expand_simple<T, MODE><<<dim3(tiles, a.p.H), 256, smem, s>>>(a);
-  return check_launch("k_expand_simple");
+template <class T>
+static int run_backward(const ll_latent_packed* p, const ExTma& tq, const ExTma& tk, const ExBwdArgs& a, void* dk_pe,
+                        cudaStream_t s) {
+  const int nqk = a.nn + a.nr;
+  if (p->Tq) {
+    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 12 * 8 + 16;
+    LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dq<T>), smem));
+    LL_TRY(launch_pdl("k_ex_dq", k_ex_dq<T>, dim3(p->Tq / 128 + p->B, p->H), dim3(kExThreads), smem, s, tq, a));
+  }
+  if (p->Tk) {
+    const int smem = 1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 6) * 8 + 16;
+    LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dkv<T>), smem));
+    LL_TRY(launch_pdl("k_ex_dkv", k_ex_dkv<T>, dim3(p->Tk / 128 + p->B, p->H), dim3(kExThreads), smem, s, tk, a));
+    const int64_t n = (int64_t)p->Tk * p->d_r;
+    if (n)
+      LL_TRY(launch_pdl("k_ex_sum_heads", k_ex_sum_heads<T>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s,
+                        (const float*)a.dkpe, p->H, n, static_cast<T*>(dk_pe)));
+  }
+  return LL_OK;
+}
+
+static size_t backward_floats(const ll_latent_packed* p) {
+  return ((size_t)p->H * p->Tk * p->d_r + 63) / 64 * 64 + (size_t)p->H * p->Tq;
 }
 
 }  // namespace ll
@@ -630,42 +993,57 @@ int ll_latent_forward(const ll_latent_packed* p, void* out, float* lse, void* st
 }
 
 size_t ll_latent_backward_workspace_bytes(const ll_latent_packed* p) {
-  if (check_packed(p) != LL_OK) return 0;
-  return (size_t)p->H * p->Tk * p->d_r * 4 + 256;
+  if (!p || p->H <= 0 || p->Tk < 0 || p->Tq < 0 || p->d_r < 0) return 0;
+  return backward_floats(p) * 4 + 256;
 }
 
 int ll_latent_backward(const ll_latent_packed* p, const void* g, int64_t g_stride_t, int64_t g_stride_h,
                        const void* out, const float* lse, void* dq, void* dk_nope, void* dk_pe, void* dv,
                        void* workspace, size_t workspace_bytes, void* stream) {
   LL_TRY(check_packed(p));
-  if (p->B == 0) return LL_OK;
+  if (p->B == 0 || (p->Tq == 0 && p->Tk == 0)) return LL_OK;
+  auto bad = [](const void* x) { return !x || (reinterpret_cast<uintptr_t>(x) & 15); };
+  if (p->Tq && (bad16(g, g_stride_t, g_stride_h) || bad(out) || !lse || bad(dq))) return LL_ERR_ARG;
+  if (p->Tk && (bad(dk_nope) || bad(dv) || (p->d_r && bad(dk_pe)))) return LL_ERR_ARG;
+  if (bad(workspace)) return LL_ERR_ARG;
   if (workspace_bytes < ll_latent_backward_workspace_bytes(p)) return LL_ERR_WORKSPACE;
   LL_TRY(check_arch());
   LL_STREAM(stream);
   g_launch_count = 0;
-  ExpandArgs a{};
-  a.p = *p;
+  ExTma tq, tk;
+  LL_TRY(packed_maps(&tq, p));
+  LL_TRY(packed_maps(&tk, p, kExQ));
+  if (p->Tq) {
+    const CUtensorMapDataType dt = p->dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    LL_TRY(rows_map(&tq.g, dt, g, p->Tq, g_stride_t, p->H, g_stride_h, p->d_v));
+    LL_TRY(rows_map(&tk.g, dt, g, p->Tq, g_stride_t, p->H, g_stride_h, p->d_v, kExQ));
+  }
+  ExBwdArgs a{};
+  a.cu_q = p->cu_q;
+  a.cu_k = p->cu_k;
   a.g = g;
+  a.o = out;
   a.g_t = g_stride_t;
   a.g_h = g_stride_h;
-  a.o = out;
-  a.lse_in = lse;
+  a.lse = lse;
+  a.dkpe = static_cast<float*>(workspace);
+  a.delta = a.dkpe + ((size_t)p->H * p->Tk * p->d_r + 63) / 64 * 64;
   a.dq = dq;
   a.dk = dk_nope;
-  a.dkpe = dk_pe;
   a.dv = dv;
-  a.dkpe_ws = static_cast<float*>(workspace);
-  const int64_t n = (int64_t)p->Tk * p->d_r;
-  if (p->dtype == 1) {
-    LL_TRY((launch_simple<__nv_bfloat16, 1>(a, s)));
-    LL_TRY((launch_simple<__nv_bfloat16, 2>(a, s)));
-    if (n) k_sum_heads<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a.dkpe_ws, p->H, n, static_cast<__nv_bfloat16*>(dk_pe));
-  } else {
-    LL_TRY((launch_simple<__half, 1>(a, s)));
-    LL_TRY((launch_simple<__half, 2>(a, s)));
-    if (n) k_sum_heads<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a.dkpe_ws, p->H, n, static_cast<__half*>(dk_pe));
-  }
-  return check_launch("k_sum_heads");
+  a.B = p->B;
+  a.Tq = p->Tq;
+  a.Tk = p->Tk;
+  a.H = p->H;
+  a.nn = p->d_n / 64;
+  a.nr = p->d_r / 64;
+  a.nv = p->d_v / 64;
+  a.causal = p->causal;
+  a.scale = p->scale;
+  a.scale_log2 = p->scale * 1.4426950408889634f;
+  a.st = latent_status();
+  if (!a.st) return LL_ERR_CUDA;
+  return p->dtype == 1 ? run_backward<__nv_bfloat16>(p, tq, tk, a, dk_pe, s) : run_backward<__half>(p, tq, tk, a, dk_pe, s);
 }
 
 }  // extern "C"

@@ -96,16 +96,17 @@ LL_DEV void seq_range(const int32_t* cu, int b, int total, int& lo, int& hi) {
   hi = min(max(cu[b + 1], lo), total);
 }
 
-// The tile-th tile of `rows` rows over all sequences, counted from the last one, for a whole warp:
-// true and (b, first row within the sequence) when there is one. Lanes scan 32 sequences at a time.
-// Counting from the end starts each sequence's causal tiles with the longest, so the short ones
-// fill the launch's tail.
-LL_DEV bool find_tile_from_end(const int32_t* cu, int B, int total, int rows, int tile, int& b, int& row0) {
+// The tile-th tile of `rows` rows over all sequences, counted from the first or (FROM_END) from the last
+// one, for a whole warp: true and (b, first row within the sequence) when there is one. Lanes scan 32
+// sequences at a time. The causal kernels count from the side on which a sequence's tiles are longest, so
+// that the short ones fill the launch's tail.
+template <bool FROM_END>
+LL_DEV bool find_tile(const int32_t* cu, int B, int total, int rows, int tile, int& b, int& row0) {
   const int lane = threadIdx.x & 31;
-  for (int hi_b = B; hi_b > 0; hi_b -= 32) {
-    const int bb = hi_b - 1 - lane;
+  for (int b0 = 0; b0 < B; b0 += 32) {
+    const int bb = FROM_END ? B - 1 - b0 - lane : b0 + lane;
     int n = 0;
-    if (bb >= 0) {
+    if (bb >= 0 && bb < B) {
       int lo, hi;
       seq_range(cu, bb, total, lo, hi);
       n = (hi - lo + rows - 1) / rows;
@@ -118,11 +119,11 @@ LL_DEV bool find_tile_from_end(const int32_t* cu, int B, int total, int rows, in
     }
     const int all = __shfl_sync(0xffffffffu, sum, 31);
     if (tile < all) {
-      const uint32_t hit = __ballot_sync(0xffffffffu, tile < sum);
-      const int src = __ffs(hit) - 1;
-      b = hi_b - 1 - src;
+      const int src = __ffs(__ballot_sync(0xffffffffu, tile < sum)) - 1;
       const int end = __shfl_sync(0xffffffffu, sum, src), cnt = __shfl_sync(0xffffffffu, n, src);
-      row0 = (cnt - 1 - (tile - (end - cnt))) * rows;
+      const int at = tile - (end - cnt);
+      b = __shfl_sync(0xffffffffu, bb, src);
+      row0 = (FROM_END ? cnt - 1 - at : at) * rows;
       return true;
     }
     tile -= all;
