@@ -753,13 +753,13 @@ int ll_gemm_bf16_sum2(int M, int N, const void* A0, int K0, int64_t lda0, const 
 int ll_gemm_bf16_heads(int T, int H, int N, int K, const void* x, int64_t x_stride_t, int64_t x_stride_h,
                        const void* W, int64_t w_stride_h, int64_t ldw, int w_nk, void* y, int64_t y_stride_t,
                        int64_t y_stride_h, void* stream) {
-  if (T < 0 || H < 0 || N <= 0 || K <= 0 || ldw < (w_nk ? K : N)) return LL_ERR_ARG;
+  if (T < 0 || H < 0 || N <= 0 || K <= 0 || ldw <= 0) return LL_ERR_ARG;
   if (T == 0 || H == 0) return LL_OK;
   if (!x || !W || !y) return LL_ERR_ARG;
   if ((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(W) | reinterpret_cast<uintptr_t>(y)) % 16)
     return LL_ERR_ARG;
   if (x_stride_t % 8 || x_stride_h % 8 || w_stride_h % 8 || ldw % 8 || y_stride_t % 8 || y_stride_h % 8) return LL_ERR_ARG;
-  if (x_stride_t < K || x_stride_h < 8 || w_stride_h < 8 || y_stride_t < N || (H > 1 && y_stride_h < 8)) return LL_ERR_ARG;
+  if (x_stride_t <= 0 || x_stride_h <= 0 || w_stride_h <= 0 || y_stride_t <= 0 || y_stride_h <= 0) return LL_ERR_ARG;
   if ((int64_t)((T + 127) / 128) * ((N + 31) / 32) * H > INT32_MAX) return LL_ERR_ARG;
   LL_TRY(check_arch());
   LL_STREAM(stream);

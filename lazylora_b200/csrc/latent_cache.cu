@@ -152,8 +152,8 @@ int ll_latent_append(const void* kv, int64_t kv_stride, const int64_t* slots, co
                      int64_t q_stride_t, int64_t q_stride_h, int H, void* q_out, int64_t qo_stride_t,
                      int64_t qo_stride_h, void* stream) {
   if (T < 0 || d_c <= 0 || d_c % 16 || d_r < 0 || d_r % 16 || (dtype != 1 && dtype != 2) || H < 0) return LL_ERR_ARG;
-  if (pages <= 0 || page_size <= 0 || table_rows <= 0 || row_stride < d_c + d_r ||
-      page_stride < (int64_t)page_size * row_stride)
+  if (pages <= 0 || page_size <= 0 || table_rows <= 0 || (page_size > 1 && row_stride < d_c + d_r) ||
+      (pages > 1 && page_stride < d_c + d_r))
     return LL_ERR_ARG;
   if (!q_pe) H = 0;
   if (T == 0) return LL_OK;

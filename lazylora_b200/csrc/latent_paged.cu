@@ -610,8 +610,8 @@ int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_strid
   if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(cache) | reinterpret_cast<uintptr_t>(out) |
        reinterpret_cast<uintptr_t>(workspace)) & 15)
     return LL_ERR_ARG;
-  if (q_stride_b % 8 || q_stride_row % 8 || q_stride_row < D || q_stride_b < D || page_stride % 8 || row_stride % 8 ||
-      row_stride < D || page_stride < D || table_stride < 0)
+  if (q_stride_b % 8 || q_stride_row % 8 || q_stride_b <= 0 || q_stride_row <= 0 || page_stride % 8 || row_stride % 8 ||
+      row_stride < D || (pages > 1 && page_stride < D) || page_stride <= 0 || table_stride < 0)
     return LL_ERR_ARG;
   if (workspace_bytes < ll_paged_latent_workspace_bytes(B, Tq, H, d_c)) return LL_ERR_WORKSPACE;
   LL_TRY(check_arch());
