@@ -35,7 +35,8 @@
 
 namespace ll {
 
-constexpr int kPgThreads = 192;
+constexpr int kPgSoft = 256;           // softmax threads: warps 0-7; warp 8: TMA, warp 9: MMA
+constexpr int kPgThreads = kPgSoft + 64;
 constexpr int kPgKeys = 64;
 constexpr float kPgSlack = 8.f;        // log2 of how far a score may pass its row's reference
 constexpr float kPgNone = -1e30f;      // reference of a row that has seen no key
@@ -47,7 +48,7 @@ struct PagedArgs {
   float* lse;
   float* part;        // [G * 2][RT][NT][d_c] unnormalised pieces
   float* part_ml;     // [G * 2][RT][2][NT] their references (log2) and sums
-  int64_t* starts;    // [B + 1] tiles before each sequence; last: tiles of a range
+  int* starts;        // [B + 1] weight before each sequence; last: weight of a range
   int64_t bt_stride;
   int pages, page_size, max_pages, B, Tq, H, rows, RT, G, nc, nchunk;   // chunks of 64: of d_c, of d_c + d_r
   float scale_log2;
@@ -59,33 +60,42 @@ struct PagedTma {
 };
 
 LL_DEV int paged_len(const PagedArgs& a, int b) {
-  return (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * a.page_size);
+  return min(max(a.lens[b], 0), a.max_pages * a.page_size);      // (the host checks that this is an int)
 }
 // A sequence without keys still has one (masked) tile, which writes its zeros.
 LL_DEV int paged_tiles(int len) { return max(1, (len - 1) / kPgKeys + 1); }
+// What a sequence weighs in the deal: its tiles, and before them the time that starting and ending it
+// costs (query load, first maxima, output), which measured about two tiles.
+constexpr int kPgStart = 2;
+LL_DEV int paged_weight(int len) { return paged_tiles(len) + kPgStart; }
 
-// tcgen05.ld of 16 lanes x 8 columns twice: threads 0-15 take columns taddr .. + 7, threads 16-31
-// columns taddr + SPLIT .. + 7 of the same lanes.
+// tcgen05.ld of 16 lanes x 8 (or 4) columns twice: threads 0-15 take columns taddr .., threads 16-31
+// columns taddr + SPLIT .. of the same lanes.
 template <int SPLIT>
 LL_DEV void tmem_ld_16x2_8(uint32_t taddr, uint32_t* r) {
   asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8], %9;"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
                : "r"(taddr), "n"(SPLIT));
 }
-
-// A softmax thread's NH values of S^T.
-template <int NH>
-LL_DEV void load_scores(uint32_t taddr, float (&v)[NH]) {
-  uint32_t raw[NH];
+template <int SPLIT>
+LL_DEV void tmem_ld_16x2_4(uint32_t taddr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.16x32bx2.x4.b32 {%0,%1,%2,%3}, [%4], %5;"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(taddr), "n"(SPLIT));
+}
+// A softmax thread's NQ values of S^T.
+template <int NQ>
+LL_DEV void load_scores(uint32_t taddr, float (&v)[NQ]) {
+  uint32_t raw[NQ];
 #pragma unroll
-  for (int c = 0; c < NH; c += 8) tmem_ld_16x2_8<NH>(taddr + c, raw + c);
+  for (int c = 0; c + 8 <= NQ; c += 8) tmem_ld_16x2_8<NQ>(taddr + c, raw + c);
+  if constexpr (NQ % 8) tmem_ld_16x2_4<NQ>(taddr + NQ - 4, raw + NQ - 4);
   tmem_ld_wait();
 #pragma unroll
-  for (int c = 0; c < NH; c += 8)
-    asm volatile("" : "+r"(raw[c]), "+r"(raw[c + 1]), "+r"(raw[c + 2]), "+r"(raw[c + 3]), "+r"(raw[c + 4]),
-                 "+r"(raw[c + 5]), "+r"(raw[c + 6]), "+r"(raw[c + 7])::"memory");
+  for (int c = 0; c < NQ; c += 4)
+    asm volatile("" : "+r"(raw[c]), "+r"(raw[c + 1]), "+r"(raw[c + 2]), "+r"(raw[c + 3])::"memory");
 #pragma unroll
-  for (int c = 0; c < NH; c++) v[c] = __uint_as_float(raw[c]);
+  for (int c = 0; c < NQ; c++) v[c] = __uint_as_float(raw[c]);
 }
 
 // Folds N values a thread across the 16 lanes of its half warp, halving the values a lane carries at each
@@ -114,12 +124,12 @@ LL_DEV int fold16(float* v, int lane, Op op) {
   }
 }
 
-// Barrier 1 of the 128 softmax threads, with a vote.
+// Barrier 1 of the softmax threads, with a vote.
 LL_DEV bool softmax_any(bool p) {
   uint32_t r;
   asm volatile(
       "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 128, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      "bar.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
       : "=r"(r)
       : "r"((uint32_t)p)
       : "memory");
@@ -128,9 +138,8 @@ LL_DEV bool softmax_any(bool p) {
 
 // The pieces [j, j_end) of sequence b, one after another, that make up a CTA's range of tiles.
 struct PagedWalk {
-  int64_t left;
-  int b, j, n, len;
-  LL_DEV void init(const PagedArgs& a, int b0, int j0, int64_t count) {
+  int left, b, j, n, len;
+  LL_DEV void init(const PagedArgs& a, int b0, int j0, int count) {
     left = count;
     b = b0;
     j = j0;
@@ -140,7 +149,7 @@ struct PagedWalk {
     len = paged_len(a, b);
     n = paged_tiles(len);
   }
-  LL_DEV int end() const { return (int)min((int64_t)n, j + left); }
+  LL_DEV int end() const { return min(n, j + left); }
   LL_DEV void next(const PagedArgs& a) {
     left -= end() - j;
     b++;
@@ -151,7 +160,7 @@ struct PagedWalk {
 
 template <class T, int NT>
 __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__ PagedTma tm, const PagedArgs a) {
-  constexpr int NH = NT / 2;             // rows of a softmax thread
+  constexpr int NQ = NT / 4;             // query rows of a softmax thread
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int nchunk = a.nchunk, group_bytes = nchunk * 1024, tile_bytes = 8 * group_bytes;
@@ -163,7 +172,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
            *p_ready = bars + 8, *pv_done = bars + 9, *o_free = bars + 10, *drain = bars + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* s_start = reinterpret_cast<int*>(tmem_slot + 2);                // b0, j0, count, per
+  int* s_start = reinterpret_cast<int*>(tmem_slot + 2);        // first sequence, first tile of it, tiles before, after
   float* s_red = reinterpret_cast<float*>(tmem_slot + 8);              // [4 warps][64]
   float* s_col = s_red + 256;                                          // [64] a factor per row
   float* s_ref = s_col + 64;                                           // [64] the rows' references
@@ -171,12 +180,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   const int g = blockIdx.x / a.RT, rt = blockIdx.x % a.RT;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 12; i++) mbar_init(&bars[i], i == 8 || i == 10 ? 4 : 1);
+    for (int i = 0; i < 12; i++) mbar_init(&bars[i], i == 8 || i == 10 ? kPgSoft / 32 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 5) tmem_alloc(tmem_slot, 512);
-  if (warp == 4 && lane == 0) {
+  if (warp == 9) tmem_alloc(tmem_slot, 512);
+  if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&tm.q);
     tma_prefetch_desc(&tm.kv);
   }
@@ -184,42 +193,46 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   if (warp == 0) {
     // the range of this CTA: each lane sums a run of consecutive sequences
     const int run = (a.B + 31) / 32, b_lo = min(lane * run, a.B), b_hi = min(b_lo + run, a.B);
-    int64_t mine = 0;
-    for (int b = b_lo; b < b_hi; b++) mine += paged_tiles(paged_len(a, b));
-    int64_t sum = mine;
+    int mine = 0;
+#pragma unroll 4
+    for (int b = b_lo; b < b_hi; b++) mine += paged_weight(paged_len(a, b));
+    int sum = mine;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
-      const int64_t v = __shfl_up_sync(0xffffffffu, sum, off);
+      const int v = __shfl_up_sync(0xffffffffu, sum, off);
       if (lane >= off) sum += v;
     }
-    const int64_t total = __shfl_sync(0xffffffffu, sum, 31), per = (total + a.G - 1) / a.G, first = g * per;
-    if (lane == 0) s_start[2] = (int)max((int64_t)0, min(per, total - first));
-    if (blockIdx.x == 0) {
-      int64_t at = sum - mine;
+    const int total = __shfl_sync(0xffffffffu, sum, 31), per = (total + a.G - 1) / a.G;
+    const int first = min((int64_t)g * per, (int64_t)total), last = min((int64_t)first + per, (int64_t)total);
+    if (lane == 0) {
+      s_start[2] = s_start[3] = total - kPgStart * a.B;      // tiles before `first`, before `last`
+      if (blockIdx.x == 0) a.starts[a.B] = per;
+    }
+    __syncwarp();
+    int at = sum - mine;
+    if (blockIdx.x == 0 || (first < sum && last >= at))
       for (int b = b_lo; b < b_hi; b++) {
-        a.starts[b] = at;
-        at += paged_tiles(paged_len(a, b));
+        const int n = paged_tiles(paged_len(a, b)), before = at - kPgStart * b, end = at + n + kPgStart;
+        if (blockIdx.x == 0) a.starts[b] = at;
+        if (first >= at && first < end) {
+          s_start[0] = b;
+          s_start[1] = max(0, first - at - kPgStart);
+          s_start[2] = before + s_start[1];
+        }
+        if (last >= at && last < end) s_start[3] = before + max(0, last - at - kPgStart);
+        at = end;
       }
-      if (lane == 0) a.starts[a.B] = per;
-    }
-    if (first >= sum - mine && first < sum) {
-      int64_t at = sum - mine;
-      int b = b_lo;
-      for (int n; at + (n = paged_tiles(paged_len(a, b))) <= first; b++) at += n;
-      s_start[0] = b;
-      s_start[1] = (int)(first - at);
-    }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   pdl_launch_next();
   const uint32_t tmem = *tmem_slot, tmem_s = tmem + 256;
-  const int count = s_start[2];
+  const int count = s_start[3] - s_start[2];
   PagedWalk w;
   w.init(a, s_start[0], s_start[1], count);
 
-  if (warp == 4) {
+  if (warp == 8) {
     // ------------------------------------------------------------------------------- TMA
     // Lane i takes the tile's group i of eight keys: it looks its page up while the stage is still in
     // use, then issues its own box.
@@ -261,7 +274,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     if (n >= 2) mbar_wait_sleep(&kv_full[n & 1], ((n - 2) >> 1) & 1, &keep, a.st, 84, 64);
     if (q_loads >= 1) mbar_wait_sleep(q_full, (q_loads - 1) & 1, &keep, a.st, 85, 64);
     __syncwarp();
-  } else if (warp == 5) {
+  } else if (warp == 9) {
     // ------------------------------------------------------------------------------- MMA
     // The whole warp runs the loop (so that descriptors stay in uniform registers), one elected
     // lane issues. S^T of tile n + 1 goes ahead of tile n's second product when its tile has already
@@ -279,8 +292,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     long long t0 = clock64();
     while (pv < (uint32_t)count) {
       bool did = false;
-      if (qk < (uint32_t)count && qk - pv <= 1 && mbar_try_wait(&kv_full[qk & 1], (qk >> 1) & 1) &&
-          (j != w.j || mbar_try_wait(q_full, seg & 1))) {
+      if (qk < (uint32_t)count && qk == pv && mbar_test(&kv_full[qk & 1], (qk >> 1) & 1) &&
+          (j != w.j || mbar_test(q_full, seg & 1))) {
         tc_fence_after();
         const uint32_t at = tmem_s + (qk & 1) * 64, k0 = k_d.lo + (qk & 1) * tile16;
         if (lead) {
@@ -301,7 +314,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         did = true;
       }
       const bool first = first_bits >> (pv & 1) & 1;
-      if (pv < qk && mbar_try_wait(p_ready, pv & 1) && (!first || seg_pv == 0 || mbar_try_wait(o_free, (seg_pv - 1) & 1))) {
+      if (pv < qk && mbar_test(p_ready, pv & 1) && (!first || seg_pv == 0 || mbar_test(o_free, (seg_pv - 1) & 1))) {
         tc_fence_after();
         const uint32_t v0 = v_d.lo + (pv & 1) * tile16;
         if (lead) {
@@ -336,54 +349,55 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     // ------------------------------------------------- softmax, rescaling and the outputs
     // A wait that ran out does not leave the loops: the other waits then return at once, every
     // barrier still meets all 128 threads, and the results are void (the status says so).
-    const int hh = lane / 16, key_in = warp * 16 + lane % 16;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    const int t0 = (rt * NT + hh * NH) / a.H, h0 = (rt * NT + hh * NH) % a.H;
+    const int quarter = warp % 4, side = warp / 4, key_in = quarter * 16 + lane % 16;
+    const int r0 = (side * 2 + lane / 16) * NQ;          // the thread's first query row in the tile
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const int t0 = (rt * NT + r0) / a.H, h0 = (rt * NT + r0) % a.H;
     uint8_t* p_row = s_p + (key_in / 8) * 1024 + (key_in % 8) * 128;
     uint32_t n = 0;
     for (; w.left > 0; w.next(a)) {
       const int j0 = w.j, j1 = w.end();
-      float ref[NH], l[NH];
+      float ref[NQ], l[NQ];
 #pragma unroll
-      for (int c = 0; c < NH; c++) { ref[c] = kPgNone; l[c] = 0.f; }
+      for (int c = 0; c < NQ; c++) { ref[c] = kPgNone; l[c] = 0.f; }
       if (threadIdx.x < NT) s_ref[threadIdx.x] = kPgNone;
       for (int j = j0; j < j1; j++, n++) {
         mbar_wait(&s_full[n & 1], (n >> 1) & 1, abort_flag, a.st, 91);
         tc_fence_after();
-        const uint32_t s_at = tmem_s + (n & 1) * 64 + lanes;
+        const uint32_t s_at = tmem_s + (n & 1) * 64 + side * 2 * NQ + lanes;
         const int k0 = j * kPgKeys, key = k0 + key_in;
         const bool inside = k0 + kPgKeys <= w.len - a.Tq + 1;       // every row sees every key
         // hides the keys past each row's last one (row (t, h) sees w.len - Tq + 1 + t of them)
-        auto mask = [&](float (&x)[NH]) {
+        auto mask = [&](float (&x)[NQ]) {
           int h = h0, see = w.len - a.Tq + 1 + t0;
 #pragma unroll
-          for (int c = 0; c < NH; c++) {
+          for (int c = 0; c < NQ; c++) {
             if (key >= see) x[c] = -INFINITY;
             if (++h == a.H) { h = 0; see++; }
           }
         };
-        float v[NH];
-        load_scores<NH>(s_at, v);
+        float v[NQ];
+        load_scores<NQ>(s_at, v);
 #pragma unroll
-        for (int c = 0; c < NH; c++) v[c] = fmaf(v[c], a.scale_log2, -ref[c]);
+        for (int c = 0; c < NQ; c++) v[c] = fmaf(v[c], a.scale_log2, -ref[c]);
         if (!inside) mask(v);
         float top = v[0];
 #pragma unroll
-        for (int c = 1; c < NH; c++) top = fmaxf(top, v[c]);
+        for (int c = 1; c < NQ; c++) top = fmaxf(top, v[c]);
         const bool slow = softmax_any(top > kPgSlack);
         if (slow) {
           // new references: each row's maximum so far
-          load_scores<NH>(s_at, v);
+          load_scores<NQ>(s_at, v);
 #pragma unroll
-          for (int c = 0; c < NH; c++) v[c] *= a.scale_log2;
+          for (int c = 0; c < NQ; c++) v[c] *= a.scale_log2;
           if (!inside) mask(v);
-          float x[NH];
+          float x[NQ];
 #pragma unroll
-          for (int c = 0; c < NH; c++) x[c] = v[c];
-          const int c0 = hh * NH + fold16<NH, 8>(x, lane, [](float p, float q) { return fmaxf(p, q); });
+          for (int c = 0; c < NQ; c++) x[c] = v[c];
+          const int c0 = r0 + fold16<NQ, 8>(x, lane, [](float p, float q) { return fmaxf(p, q); });
 #pragma unroll
-          for (int c = 0; c < fold_left(NH); c++) s_red[warp * 64 + c0 + c] = x[c];
-          named_bar_sync(1, 128);
+          for (int c = 0; c < fold_left(NQ); c++) s_red[quarter * 64 + c0 + c] = x[c];
+          named_bar_sync(1, kPgSoft);
           if (threadIdx.x < NT) {
             const int r = threadIdx.x;
             const float was = s_ref[r];
@@ -391,46 +405,45 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
             s_ref[r] = now;
             s_col[r] = ex2(was - now);
           }
-          named_bar_sync(1, 128);
+          named_bar_sync(1, kPgSoft);
 #pragma unroll
-          for (int c = 0; c < NH; c++) {
-            ref[c] = s_ref[hh * NH + c];
+          for (int c = 0; c < NQ; c++) {
+            ref[c] = s_ref[r0 + c];
             v[c] -= ref[c];
-            l[c] *= s_col[hh * NH + c];
+            l[c] *= s_col[r0 + c];
           }
         }
 #pragma unroll
-        for (int c = 0; c < NH; c++) {
+        for (int c = 0; c < NQ; c++) {
           v[c] = ex2(v[c]);
           l[c] += v[c];
         }
         if (n > 0) mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.st, 92);      // P and O are free
         if (slow && j > j0) {
           tc_fence_after();
-          for (int mt = 0; mt < a.nc / 2; mt++)
-            for (int c = 0; c < NT; c += 16) {
-              float o[16];
-              const uint32_t at = tmem + mt * NT + c + lanes;
-              tmem_ld16(at, o);
-              tmem_ld_wait();
-              uint32_t u[16];
+          for (int i = side; i < a.nc / 2 * (NT / 16); i += 2) {
+            const int c = i % (NT / 16) * 16;
+            const uint32_t at = tmem + i / (NT / 16) * NT + c + lanes;
+            float o[16];
+            tmem_ld16(at, o);
+            tmem_ld_wait();
+            uint32_t u[16];
 #pragma unroll
-              for (int i = 0; i < 16; i++) u[i] = __float_as_uint(o[i] * s_col[c + i]);
-              tmem_st16(at, u);
-            }
+            for (int k = 0; k < 16; k++) u[k] = __float_as_uint(o[k] * s_col[c + k]);
+            tmem_st16(at, u);
+          }
           tmem_st_wait();
         }
 #pragma unroll
-        for (int c = 0; c < NH; c += 8) {
-          const int chunk = (hh * NH + c) / 8;
-          *reinterpret_cast<uint4*>(p_row + ((chunk ^ (key_in % 8)) * 16)) =
-              make_uint4(Num<T>::pack(v[c], v[c + 1]), Num<T>::pack(v[c + 2], v[c + 3]), Num<T>::pack(v[c + 4], v[c + 5]),
-                         Num<T>::pack(v[c + 6], v[c + 7]));
+        for (int c = 0; c < NQ; c += 4) {
+          const int chunk = (r0 + c) / 8, half = (r0 + c) / 4 % 2;
+          *reinterpret_cast<uint2*>(p_row + ((chunk ^ (key_in % 8)) * 16) + half * 8) =
+              make_uint2(Num<T>::pack(v[c], v[c + 1]), Num<T>::pack(v[c + 2], v[c + 3]));
         }
         const int valid = w.len - k0;
         if (valid < kPgKeys) {
           const int from = max(valid, 0), per_row = a.nc * 8;
-          for (int i = threadIdx.x; i < (kPgKeys - from) * per_row; i += 128) {
+          for (int i = threadIdx.x; i < (kPgKeys - from) * per_row; i += kPgSoft) {
             const int r = from + i / per_row, c = i % per_row;
             *reinterpret_cast<uint4*>(s_kv + (n & 1) * tile_bytes + (r / 8) * group_bytes + (c / 8) * 1024 + (r % 8) * 128 +
                                       (c % 8) * 16) = make_uint4(0, 0, 0, 0);
@@ -442,10 +455,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         if (lane == 0) mbar_arrive(p_ready);
       }
       // the piece's sums over its keys, in a fixed order
-      const int c0 = hh * NH + fold16<NH, 8>(l, lane, [](float p, float q) { return p + q; });
+      const int c0 = r0 + fold16<NQ, 8>(l, lane, [](float p, float q) { return p + q; });
 #pragma unroll
-      for (int c = 0; c < fold_left(NH); c++) s_red[warp * 64 + c0 + c] = l[c];
-      named_bar_sync(1, 128);
+      for (int c = 0; c < fold_left(NQ); c++) s_red[quarter * 64 + c0 + c] = l[c];
+      named_bar_sync(1, kPgSoft);
       const bool whole = j0 == 0 && j1 == w.n;
       const int64_t slot = ((int64_t)g * 2 + (n == (uint32_t)(j1 - j0) ? 0 : 1)) * a.RT + rt;
       if (threadIdx.x < NT) {
@@ -460,16 +473,16 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
           a.lse[(int64_t)w.b * a.rows + row] = any ? (s_ref[r] + log2f(sum)) * 0.693147180559945309f : -INFINITY;
         }
       }
-      named_bar_sync(1, 128);
+      named_bar_sync(1, kPgSoft);
       mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.st, 93);
       tc_fence_after();
       const int d_c = a.nc * 64;
-      for (int mt = 0; mt < a.nc / 2; mt++)
-        for (int c = 0; c < NT; c += 16) {
+      for (int j = side; j < a.nc / 2 * (NT / 16); j += 2) {
+          const int mt = j / (NT / 16), c = j % (NT / 16) * 16;
           float o[16];
           tmem_ld16(tmem + mt * NT + c + lanes, o);
           tmem_ld_wait();
-          const int d = mt * 128 + warp * 32 + lane;
+          const int d = mt * 128 + quarter * 32 + lane;
           if (!whole) {
             float* dst = a.part + (slot * NT + c) * d_c + d;
 #pragma unroll
@@ -495,49 +508,60 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 5) tmem_dealloc(tmem, 512);
+  if (warp == 9) tmem_dealloc(tmem, 512);
 }
 
-// Joins a split sequence's pieces: out = sum_g 2^(m_g - M) O_g / sum_g 2^(m_g - M) l_g, in CTA order.
-// One block per query row, four values a thread, eight pieces' loads in flight; rows of whole
-// sequences are left alone.
-template <class T>
-__global__ void __launch_bounds__(128) k_paged_combine(const PagedArgs a, int NT) {
+// Joins a split sequence's pieces: out = sum_g 2^(m_g - M) O_g / sum_g 2^(m_g - M) l_g with the running
+// maximum M. One block per query row; GRP groups of 128 threads take the pieces in turn, four values a
+// thread and four pieces' loads in flight (most sequences have fewer, so that a row takes two dependent
+// rounds of loads: its range, its pieces), and are joined in order. GRP 4 where a sequence has many pieces
+// (few long ones, 37 pieces: 25 us with one group). Rows of whole sequences are left alone.
+template <class T, int GRP>
+__global__ void __launch_bounds__(128 * GRP) k_paged_combine(const PagedArgs a, int NT) {
+  __shared__ float4 s_o[GRP][128];
+  __shared__ float2 s_ml[GRP];
   const int b = blockIdx.x / a.rows, row = blockIdx.x % a.rows, rt = row / NT, r = row % NT;
+  const int grp = threadIdx.x / 128, t = threadIdx.x % 128;
   pdl_wait();
-  const int64_t before = a.starts[b], per = a.starts[a.B];
-  const int64_t last = before + paged_tiles(paged_len(a, b)) - 1;
-  const int g0 = (int)(before / per), g1 = (int)(last / per);
-  if (g0 == g1) return;
-  // a CTA's first piece is in its slot 0, its last (when another) in slot 1
-  auto slot = [&](int g) { return ((int64_t)g * 2 + (before > g * per ? 1 : 0)) * a.RT + rt; };
-  const int d_c = a.nc * 64, d = threadIdx.x * 4, n = g1 - g0 + 1, lane = threadIdx.x % 32;
-  float M = kPgNone;
-  for (int i = lane; i < n; i += 32) M = fmaxf(M, a.part_ml[slot(g0 + i) * 2 * NT + r]);
-#pragma unroll
-  for (int off = 16; off; off >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, off));
-  float L = 0.f;
+  const int before = a.starts[b], per = a.starts[a.B];
+  const int tile0 = before + kPgStart, last = tile0 + paged_tiles(paged_len(a, b)) - 1;
+  const int g0 = tile0 / per, n = last / per - g0 + 1;
+  if (n == 1) return;
+  const int d_c = a.nc * 64, d = t * 4;
+  float M = kPgNone, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < n; i0 += 8) {
-    float f[8], l[8];
-    float4 x[8];
+  auto join = [&](float m, float l, float4 x) {
+    const float now = fmaxf(M, m), f = ex2(M - now), w = ex2(m - now);
+    M = now;
+    L = L * f + w * l;
+    o.x = o.x * f + w * x.x;
+    o.y = o.y * f + w * x.y;
+    o.z = o.z * f + w * x.z;
+    o.w = o.w * f + w * x.w;
+  };
+  for (int i0 = grp; i0 < n; i0 += 4 * GRP) {
+    float m[4], l[4];
+    float4 x[4];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int64_t sl = slot(g0 + min(i0 + i, n - 1));
-      f[i] = a.part_ml[sl * 2 * NT + r];
+    for (int i = 0; i < 4; i++) {
+      // a CTA's first piece is in its slot 0, its last (when another) in slot 1
+      const int g = g0 + min(i0 + i * GRP, n - 1);
+      const int64_t sl = ((int64_t)g * 2 + (before > g * per ? 1 : 0)) * a.RT + rt;
+      m[i] = a.part_ml[sl * 2 * NT + r];
       l[i] = a.part_ml[sl * 2 * NT + NT + r];
       x[i] = d < d_c ? *reinterpret_cast<const float4*>(a.part + (sl * NT + r) * d_c + d) : o;
     }
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      if (i0 + i >= n) break;
-      const float w = ex2(f[i] - M);
-      L = fmaf(w, l[i], L);
-      o.x = fmaf(w, x[i].x, o.x);
-      o.y = fmaf(w, x[i].y, o.y);
-      o.z = fmaf(w, x[i].z, o.z);
-      o.w = fmaf(w, x[i].w, o.w);
-    }
+    for (int i = 0; i < 4; i++)
+      if (i0 + i * GRP < n) join(m[i], l[i], x[i]);
+  }
+  if (GRP > 1) {
+    s_o[grp][t] = o;
+    if (t == 0) s_ml[grp] = make_float2(M, L);
+    __syncthreads();
+    if (grp > 0) return;
+#pragma unroll
+    for (int i = 1; i < GRP; i++) join(s_ml[i].x, s_ml[i].y, s_o[i][t]);
   }
   const bool any = !(L <= 0.f);
   const float inv = any ? 1.f / L : 0.f;
@@ -545,7 +569,7 @@ __global__ void __launch_bounds__(128) k_paged_combine(const PagedArgs a, int NT
   if (d < d_c)
     *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * d_c + d) =
         make_uint2(Num<T>::pack(o.x * inv, o.y * inv), Num<T>::pack(o.z * inv, o.w * inv));
-  if (threadIdx.x == 0) a.lse[at] = any ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+  if (t == 0) a.lse[at] = any ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
 }
 
 // Row tiles of a sequence, their height (a multiple of 16, the tiles' rows nearly equal) and the
@@ -579,7 +603,9 @@ static int run_paged(const PagedTma& tm, const PagedArgs& a, int NT, cudaStream_
   else if (NT == 48) LL_TRY((launch_paged<T, 48>(tm, a, smem, s)));
   else LL_TRY((launch_paged<T, 64>(tm, a, smem, s)));
   if (a.G == 1) return LL_OK;
-  return launch_pdl("k_paged_combine", k_paged_combine<T>, dim3((unsigned)a.B * a.rows), dim3(128), 0, s, a, NT);
+  const dim3 grid((unsigned)a.B * a.rows);
+  if (a.G > 8 * a.B) return launch_pdl("k_paged_combine", k_paged_combine<T, 4>, grid, dim3(512), 0, s, a, NT);
+  return launch_pdl("k_paged_combine", k_paged_combine<T, 1>, grid, dim3(128), 0, s, a, NT);
 }
 
 }  // namespace ll
@@ -602,7 +628,8 @@ int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_strid
   if (B < 0 || Tq <= 0 || H <= 0 || d_c <= 0 || d_c % 128 || d_c > 512 || (d_r != 0 && d_r != 64) ||
       (dtype != 1 && dtype != 2) || pages <= 0 || page_size <= 0 || page_size % 8 || max_pages <= 0 || !(scale > 0.f))
     return LL_ERR_ARG;
-  if ((int64_t)Tq * H > (1 << 24) || (int64_t)B * Tq * H > INT32_MAX || (int64_t)max_pages * page_size > INT32_MAX - 64)
+  if ((int64_t)Tq * H > (1 << 24) || (int64_t)B * Tq * H > INT32_MAX || (int64_t)max_pages * page_size > INT32_MAX - 64 ||
+      (int64_t)B * ((int64_t)max_pages * page_size / kPgKeys + 1 + kPgStart) > INT32_MAX)
     return LL_ERR_ARG;
   if (B == 0) return LL_OK;
   const int D = d_c + d_r;
@@ -626,7 +653,7 @@ int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_strid
   Carver cv(workspace);
   a.part = cv.take<float>(p.part);
   a.part_ml = cv.take<float>(p.ml);
-  a.starts = cv.take<int64_t>((size_t)B + 1);
+  a.starts = cv.take<int>((size_t)B + 1);
   a.bt_stride = table_stride;
   a.pages = pages;
   a.page_size = page_size;
