@@ -512,64 +512,83 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
 }
 
 // Joins a split sequence's pieces: out = sum_g 2^(m_g - M) O_g / sum_g 2^(m_g - M) l_g with the running
-// maximum M. One block per query row; GRP groups of 128 threads take the pieces in turn, four values a
-// thread and four pieces' loads in flight (most sequences have fewer, so that a row takes two dependent
-// rounds of loads: its range, its pieces), and are joined in order. GRP 4 where a sequence has many pieces
-// (few long ones, 37 pieces: 25 us with one group). Rows of whole sequences are left alone.
-template <class T, int GRP>
+// maximum M. A block takes ROWS query rows, a thread four values of each; rows of whole sequences are left
+// alone. Bound by its two dependent rounds of loads (the sequence's range, its pieces), so the second one
+// has many in flight: with few pieces a sequence ROWS = 4 and two pieces at a time; with many (few long
+// sequences) one row, whose pieces GRP = 4 groups of threads take in turn, four at a time, and join in
+// order (37 pieces: 25 us with one group, 6 with four).
+template <class T, int GRP, int ROWS>
 __global__ void __launch_bounds__(128 * GRP) k_paged_combine(const PagedArgs a, int NT) {
+  constexpr int PC = GRP > 1 ? 4 : 2;
   __shared__ float4 s_o[GRP][128];
   __shared__ float2 s_ml[GRP];
-  const int b = blockIdx.x / a.rows, row = blockIdx.x % a.rows, rt = row / NT, r = row % NT;
+  const int blocks = (a.rows + ROWS - 1) / ROWS;             // a sequence's
+  const int b = blockIdx.x / blocks, row0 = blockIdx.x % blocks * ROWS, rt = row0 / NT, r0 = row0 % NT;
   const int grp = threadIdx.x / 128, t = threadIdx.x % 128;
   pdl_wait();
   const int before = a.starts[b], per = a.starts[a.B];
   const int tile0 = before + kPgStart, last = tile0 + paged_tiles(paged_len(a, b)) - 1;
   const int g0 = tile0 / per, n = last / per - g0 + 1;
   if (n == 1) return;
-  const int d_c = a.nc * 64, d = t * 4;
-  float M = kPgNone, L = 0.f;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto join = [&](float m, float l, float4 x) {
-    const float now = fmaxf(M, m), f = ex2(M - now), w = ex2(m - now);
-    M = now;
-    L = L * f + w * l;
-    o.x = o.x * f + w * x.x;
-    o.y = o.y * f + w * x.y;
-    o.z = o.z * f + w * x.z;
-    o.w = o.w * f + w * x.w;
-  };
-  for (int i0 = grp; i0 < n; i0 += 4 * GRP) {
-    float m[4], l[4];
-    float4 x[4];
+  const int d_c = a.nc * 64, d = min(t * 4, d_c - 4);
+  float M[ROWS], L[ROWS];
+  float4 o[ROWS];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-      // a CTA's first piece is in its slot 0, its last (when another) in slot 1
+  for (int k = 0; k < ROWS; k++) {
+    M[k] = kPgNone;
+    L[k] = 0.f;
+    o[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  auto join = [&](int k, float m, float l, float4 x) {
+    const float now = fmaxf(M[k], m), f = ex2(M[k] - now), w = ex2(m - now);
+    M[k] = now;
+    L[k] = L[k] * f + w * l;
+    o[k].x = o[k].x * f + w * x.x;
+    o[k].y = o[k].y * f + w * x.y;
+    o[k].z = o[k].z * f + w * x.z;
+    o[k].w = o[k].w * f + w * x.w;
+  };
+  for (int i0 = grp; i0 < n; i0 += PC * GRP) {
+    float m[PC][ROWS], l[PC][ROWS];
+    float4 x[PC][ROWS];
+#pragma unroll
+    for (int i = 0; i < PC; i++) {
+      // a CTA's first piece is in its slot 0, its last (when another) in slot 1; a row tile has NT rows,
+      // so rows past the sequence's last are there to be read
       const int g = g0 + min(i0 + i * GRP, n - 1);
       const int64_t sl = ((int64_t)g * 2 + (before > g * per ? 1 : 0)) * a.RT + rt;
-      m[i] = a.part_ml[sl * 2 * NT + r];
-      l[i] = a.part_ml[sl * 2 * NT + NT + r];
-      x[i] = d < d_c ? *reinterpret_cast<const float4*>(a.part + (sl * NT + r) * d_c + d) : o;
+#pragma unroll
+      for (int k = 0; k < ROWS; k++) {
+        m[i][k] = a.part_ml[sl * 2 * NT + r0 + k];
+        l[i][k] = a.part_ml[sl * 2 * NT + NT + r0 + k];
+        x[i][k] = *reinterpret_cast<const float4*>(a.part + (sl * NT + r0 + k) * d_c + d);
+      }
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-      if (i0 + i * GRP < n) join(m[i], l[i], x[i]);
+    for (int i = 0; i < PC; i++)
+      if (i0 + i * GRP < n)
+#pragma unroll
+        for (int k = 0; k < ROWS; k++) join(k, m[i][k], l[i][k], x[i][k]);
   }
-  if (GRP > 1) {
-    s_o[grp][t] = o;
-    if (t == 0) s_ml[grp] = make_float2(M, L);
+  if constexpr (GRP > 1) {
+    s_o[grp][t] = o[0];
+    if (t == 0) s_ml[grp] = make_float2(M[0], L[0]);
     __syncthreads();
     if (grp > 0) return;
 #pragma unroll
-    for (int i = 1; i < GRP; i++) join(s_ml[i].x, s_ml[i].y, s_o[i][t]);
+    for (int i = 1; i < GRP; i++) join(0, s_ml[i].x, s_ml[i].y, s_o[i][t]);
   }
-  const bool any = !(L <= 0.f);
-  const float inv = any ? 1.f / L : 0.f;
-  const int64_t at = (int64_t)b * a.rows + row;
-  if (d < d_c)
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * d_c + d) =
-        make_uint2(Num<T>::pack(o.x * inv, o.y * inv), Num<T>::pack(o.z * inv, o.w * inv));
-  if (t == 0) a.lse[at] = any ? (M + log2f(L)) * 0.693147180559945309f : -INFINITY;
+#pragma unroll
+  for (int k = 0; k < ROWS; k++) {
+    if (row0 + k >= a.rows) break;
+    const bool any = !(L[k] <= 0.f);
+    const float inv = any ? 1.f / L[k] : 0.f;
+    const int64_t at = (int64_t)b * a.rows + row0 + k;
+    if (t * 4 < d_c)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at * d_c + d) =
+          make_uint2(Num<T>::pack(o[k].x * inv, o[k].y * inv), Num<T>::pack(o[k].z * inv, o[k].w * inv));
+    if (t == 0) a.lse[at] = any ? (M[k] + log2f(L[k])) * 0.693147180559945309f : -INFINITY;
+  }
 }
 
 // Row tiles of a sequence, their height (a multiple of 16, the tiles' rows nearly equal) and the
@@ -603,9 +622,10 @@ static int run_paged(const PagedTma& tm, const PagedArgs& a, int NT, cudaStream_
   else if (NT == 48) LL_TRY((launch_paged<T, 48>(tm, a, smem, s)));
   else LL_TRY((launch_paged<T, 64>(tm, a, smem, s)));
   if (a.G == 1) return LL_OK;
-  const dim3 grid((unsigned)a.B * a.rows);
-  if (a.G > 8 * a.B) return launch_pdl("k_paged_combine", k_paged_combine<T, 4>, grid, dim3(512), 0, s, a, NT);
-  return launch_pdl("k_paged_combine", k_paged_combine<T, 1>, grid, dim3(128), 0, s, a, NT);
+  if (a.G > 8 * a.B)         // more than about eight pieces a sequence
+    return launch_pdl("k_paged_combine", k_paged_combine<T, 4, 1>, dim3((unsigned)a.B * a.rows), dim3(512), 0, s, a, NT);
+  return launch_pdl("k_paged_combine", k_paged_combine<T, 1, 4>, dim3((unsigned)a.B * ((a.rows + 3) / 4)), dim3(128), 0,
+                    s, a, NT);
 }
 
 }  // namespace ll
