@@ -12,7 +12,7 @@ namespace ll {
 // One CTA takes 256 query rows of one sequence and head as two tiles of 128 that alternate: while one
 // tile's softmax runs, the tensor cores do the other's products.
 //   S_t [128][128 keys] = Q_t K^T       (M = 128, N = 128, K = d_n + d_r)
-//   O_t [128][d_v]     += P_t V         (P_t from tensor memory, 64 columns of O an instruction)
+//   O_t [128][d_v]     += P_t V         (P_t from tensor memory)
 // Issue order per key tile i: S_0(i), O_1(i - 1), S_1(i), O_0(i). Per 256 x 128 scores at 192 / 128 that
 // is 2560 cycles of products against 2048 of exponentials (16 a cycle): the tensor cores bound it.
 // Tensor memory: S_0 | S_1 | O_0 | O_1, 128 columns each; P_t overwrites the first half of S_t.
@@ -45,13 +45,14 @@ struct ExFwdArgs {
   DevStatus* st;
 };
 
-// The ring's bookkeeping, in step on the TMA and the MMA side: operands take consecutive slots.
+// The ring's bookkeeping, in step wherever it is kept: operands take consecutive slots; a value tile, whose
+// chunks one instruction reads at a fixed distance, does not go around the end (the last slot is skipped).
 struct ExRing {
   uint32_t e = 0;      // operands so far
   int slot = 0;        // the next slot
-  LL_DEV int take(int chunks) {
-    const int s = slot;
-    slot = (slot + chunks) % kExRing;
+  LL_DEV int take(int chunks, bool values) {
+    const int s = values && slot + chunks > kExRing ? 0 : slot;
+    slot = (s + chunks) % kExRing;
     e++;
     return s;
   }
@@ -93,6 +94,41 @@ LL_DEV void zero_rows(uint8_t* ring, int slot, int chunks, int from, int t, int 
   }
 }
 
+// Writes 128 bytes of each of a warp's 32 rows (lane = row, w its 32 words) through 4 KB of shared memory, so
+// that eight lanes write a row's 128 bytes at once: rows apart by a token's stride, written 16 bytes a row
+// and instruction, took 4000 cycles a 128 x 128 tile. rows: how many of the 32 exist; stride in bytes.
+LL_DEV void store_rows(uint8_t* stage, const uint32_t* w, int lane, int rows, uint8_t* dst, int64_t stride) {
+#pragma unroll
+  for (int c = 0; c < 8; c++)
+    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
+        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const int r = i * 4 + lane / 8, c = lane % 8;
+    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) * 16));
+    if (r < rows) *reinterpret_cast<uint4*>(dst + r * stride + c * 16) = v;
+  }
+  __syncwarp();
+}
+// 64 columns of an accumulator (zeros where nothing was summed), times f, as 32 words of the 16-bit type.
+template <class T>
+LL_DEV void load_acc64(uint32_t at, bool any, float f, uint32_t* w) {
+  if (any) {
+    uint32_t o[64];
+    ld32(at, o);
+    ld32(at + 32, o + 32);
+    tmem_ld_wait();
+    ld32_ready(o);
+    ld32_ready(o + 32);
+#pragma unroll
+    for (int k = 0; k < 32; k++) w[k] = Num<T>::pack(__uint_as_float(o[2 * k]) * f, __uint_as_float(o[2 * k + 1]) * f);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 32; k++) w[k] = 0;
+  }
+}
+
 // Key tiles of 128 that the query tile of `rows` rows from `q0` on sees.
 LL_DEV int key_tiles(int q0, int rows, int nq, int nk, bool causal) {
   if (q0 >= nq) return 0;
@@ -110,15 +146,14 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
   uint8_t* ring = s_q + 2 * nqk * kExChunk;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kExRing * kExChunk);
   uint64_t *full = bars, *rel = full + kExOps, *q_full = rel + kExOps, *s_full = q_full + 2, *p_ready = s_full + 2,
-           *pv_done = p_ready + 2, *drain = pv_done + 2;
+           *pv_done = p_ready + 4, *drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kExOps + 4; i++) mbar_init(&bars[i], 1);
-    mbar_init(&p_ready[0], 4);
-    mbar_init(&p_ready[1], 4);
+    for (int i = 0; i < 4; i++) mbar_init(&p_ready[i], 4);
     mbar_init(&pv_done[0], 1);
     mbar_init(&pv_done[1], 1);
     mbar_init(drain, 1);
@@ -154,38 +189,36 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
    if (warp == 8) {
     // ------------------------------------------------------------------------------- TMA
-    if (lane == 0 && n > 0) {
+    // Lane c brings chunk c: boxes that one thread issues follow each other about 350 cycles apart.
+    if (n > 0) {
       ExRing rg;
       bool ok = true;
-      int owner[kExRing];                      // operand that last took a slot
-#pragma unroll
-      for (int i = 0; i < kExRing; i++) owner[i] = -1;
+      int owner = -1;                          // lane s: the operand that last took slot s
       auto load = [&](bool key, int row) {
-        const int chunks = key ? nqk : a.nv, e = rg.e;
-        int need = -1;
-#pragma unroll
-        for (int i = 0; i < kExRing; i++)
-          if ((i - rg.slot + kExRing) % kExRing < chunks) {
-            need = max(need, owner[i]);
-            owner[i] = e;
-          }
-        if (need >= 0 && !mbar_wait(&rel[need % kExOps], (need / kExOps) & 1, abort_flag, a.st, 101)) return false;
-        const int s = rg.take(chunks);
-        uint64_t* bar = &full[e % kExOps];
-        mbar_arrive_expect_tx(bar, chunks * kExChunk);
-        for (int c = 0; c < chunks; c++) {
-          uint8_t* dst = ring + ((s + c) % kExRing) * kExChunk;
-          if (!key) tma_load_3d(dst, &tm.v, bar, c * 64, head, row);
-          else if (c < a.nn) tma_load_3d(dst, &tm.kn, bar, c * 64, head, row);
-          else tma_load_2d(dst, &tm.kp, bar, (c - a.nn) * 64, row);
+        const int chunks = key ? nqk : a.nv, e = rg.e, s0 = rg.take(chunks, !key);
+        const bool mine = lane < kExRing && (lane - s0 + kExRing) % kExRing < chunks;
+        const int need = __reduce_max_sync(0xffffffffu, mine ? owner : -1);
+        if (mine) owner = e;
+        if (need >= 0 && !mbar_wait(&rel[need % kExOps], (need / kExOps) & 1, abort_flag, a.st, 101)) {
+          rg.e--;
+          return false;
         }
+        uint64_t* bar = &full[e % kExOps];
+        if (lane == 0) mbar_arrive_expect_tx(bar, chunks * kExChunk);
+        __syncwarp();
+        uint8_t* dst = ring + ((s0 + lane) % kExRing) * kExChunk;
+        if (key && lane < a.nn) tma_load_3d(dst, &tm.kn, bar, lane * 64, head, row);
+        else if (key && lane < nqk) tma_load_2d(dst, &tm.kp, bar, (lane - a.nn) * 64, row);
+        else if (!key && lane < a.nv) tma_load_3d(dst, &tm.v, bar, lane * 64, head, row);
+        __syncwarp();
         return true;
       };
       for (int t = 0; t < 2; t++) {
         if ((t ? n1 : n0) > 0) {
-          mbar_arrive_expect_tx(&q_full[t], nqk * kExChunk);
-          for (int c = 0; c < nqk; c++)
-            tma_load_3d(s_q + (t * nqk + c) * kExChunk, &tm.q, &q_full[t], c * 64, head, q_lo + q0 + t * 128);
+          if (lane == 0) mbar_arrive_expect_tx(&q_full[t], nqk * kExChunk);
+          __syncwarp();
+          if (lane < nqk)
+            tma_load_3d(s_q + (t * nqk + lane) * kExChunk, &tm.q, &q_full[t], lane * 64, head, q_lo + q0 + t * 128);
         }
         if (t == 0) ok = load(true, k_lo);
       }
@@ -202,8 +235,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
     // ------------------------------------------------------------------------------- MMA
     const bool lead = elect_one();
     const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, 128, false, false);
-    const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, 64, false, true);
-    const MmaDesc q_d(smem_u32(s_q), 16, 1024), k_d(smem_u32(ring), 16, 1024), v_d(smem_u32(ring), 1024, 1024);
+    const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, a.nv * 64, false, true);
+    const MmaDesc q_d(smem_u32(s_q), 16, 1024), k_d(smem_u32(ring), 16, 1024), v_d(smem_u32(ring), kExChunk, 1024);
     bool ok = true;
     ExRing rg;                                 // operands alternate: key tile i is 2 i, value tile 2 i + 1
     int k_slot = 0, v_slot = 0;
@@ -213,7 +246,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
       if (i < n) {
         if (t == 0) {
           if (!(ok = mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 105))) break;
-          k_slot = rg.take(nqk);
+          k_slot = rg.take(nqk, false);
         }
         if (i < (t ? n1 : n0)) {
           if (i == 0 && !(ok = mbar_wait(&q_full[t], 0, abort_flag, a.st, 106))) break;
@@ -234,24 +267,26 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
           // the key tile is done with; the value tile comes next in the ring
           if (lead) mma_commit(&rel[(rg.e - 1) % kExOps]);
           if (!(ok = mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 107))) break;
-          v_slot = rg.take(a.nv);
+          v_slot = rg.take(a.nv, true);
         }
       }
       const int u = 1 - t, j = i - u;          // the other tile's outputs: O_1(i - 1), O_0(i)
       if (j < 0) continue;
       if (j < (u ? n1 : n0)) {
-        if (!(ok = mbar_wait(&p_ready[u], j & 1, abort_flag, a.st, 108))) break;
-        tc_fence_after();
-        if (lead) {
 #pragma unroll 1
-          for (int c = 0; c < a.nv; c++) {
-            const uint32_t v_lo16 = v_d.lo + ((v_slot + c) % kExRing) * (kExChunk / 16);
+        for (int half = 0; half < 2; half++) {       // P comes in halves of 64 keys
+          if (!(ok = mbar_wait(&p_ready[2 * u + half], j & 1, abort_flag, a.st, 108))) break;
+          tc_fence_after();
+          if (lead) {
+            const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16) + half * 512;
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++)
-              mma_16bit_ts(tmem + 256 + u * 128 + c * 64, tmem + u * 128 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o, j + kk);
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit_ts(tmem + 256 + u * 128, tmem + u * 128 + half * 32 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o,
+                           j + half + kk);
           }
-          mma_commit(&pv_done[u]);
         }
+        if (!ok) break;
+        if (lead) mma_commit(&pv_done[u]);
       }
       if (u == 1 && lead) mma_commit(&rel[(2 * j + 1) % kExOps]);
     }
@@ -272,8 +307,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
     bool ok = true;
     ExRing rv;
     for (int i = 0; i < tiles; i++) {
-      rv.slot = (rv.slot + nqk) % kExRing;
-      const int v_slot = rv.take(a.nv);
+      rv.take(nqk, false);
+      const int v_slot = rv.take(a.nv, true);
       if (!(ok = mbar_wait(&s_full[t], i & 1, abort_flag, a.st, 110))) break;
       tc_fence_after();
       uint32_t x[128];
@@ -312,21 +347,6 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
           }
         }
       }
-      float s[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c0 = 0; c0 < 128; c0 += 64) {
-        uint32_t w[32];
-#pragma unroll
-        for (int c = 0; c < 64; c += 2) {
-          const float u = ex2(fmaf(__uint_as_float(x[c0 + c]), a.scale_log2, -ref));
-          const float v = ex2(fmaf(__uint_as_float(x[c0 + c + 1]), a.scale_log2, -ref));
-          s[c % 4] += u;
-          s[c % 4 + 1] += v;
-          w[c / 2] = Num<T>::pack(u, v);
-        }
-        st32(s_at + c0 / 2, w);
-      }
-      l += (s[0] + s[1]) + (s[2] + s[3]);
       if (i * 128 + 128 > nk) {
         // the value rows past the sequence's end, which may hold anything, must not meet P's zeros
         const uint32_t e = 2 * i + 1;
@@ -334,36 +354,44 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
         zero_rows(ring, v_slot, a.nv, nk - i * 128, threadIdx.x % 128, 128);
         fence_async_smem();
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_ready[t]);
+      // P in two halves, so that the second one's exponentials run beside the first one's products
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+      for (int c0 = 0; c0 < 128; c0 += 64) {
+        uint32_t w[32];
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          float2 u = fma2(make_float2(__uint_as_float(x[c0 + c]), __uint_as_float(x[c0 + c + 1])),
+                          make_float2(a.scale_log2, a.scale_log2), make_float2(-ref, -ref));
+          u.x = ex2(u.x);
+          u.y = ex2(u.y);
+          sum[c / 2 % 2] = add2(sum[c / 2 % 2], u);
+          w[c / 2] = Num<T>::pack(u.x, u.y);
+        }
+        st32(s_at + c0 / 2, w);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[2 * t + c0 / 64]);
+      }
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     if (ok && tiles > 0) ok = mbar_wait(&pv_done[t], (tiles - 1) & 1, abort_flag, a.st, 113);
     tc_fence_after();
+    // the tile's products are done: its first query chunk is free as a stage, 4 KB a warp
     const bool live = !(l <= 0.f);
     const float inv = live ? 1.f / l : 0.f;
-    T* dst = static_cast<T*>(a.out) + ((int64_t)(q_lo + row) * a.H + head) * (a.nv * 64);
-    for (int c = 0; c < a.nv * 64; c += 32) {
-      uint32_t o[32];
-      if (tiles > 0) {
-        ld32(o_at + c, o);
-        tmem_ld_wait();
-        ld32_ready(o);
-      } else {
+    const int w_row = row - lane;
+    uint8_t* stage = s_q + t * nqk * kExChunk + (warp % 4) * 4096;
+    uint8_t* dst = static_cast<uint8_t*>(a.out) + ((int64_t)(q_lo + w_row) * a.H + head) * (a.nv * 128);
+    const bool summed = tiles > 0;
+    for (int c = 0; c < a.nv; c++) {
+      uint32_t w[32];
+      load_acc64<T>(o_at + c * 64, summed, inv, w);
+      if (!live)
 #pragma unroll
-        for (int k = 0; k < 32; k++) o[k] = 0;
-      }
-      if (row < nq) {
-#pragma unroll
-        for (int k = 0; k < 32; k += 8) {
-          uint32_t w[4];
-#pragma unroll
-          for (int z = 0; z < 4; z++)
-            w[z] = Num<T>::pack(live ? __uint_as_float(o[k + 2 * z]) * inv : 0.f, live ? __uint_as_float(o[k + 2 * z + 1]) * inv : 0.f);
-          *reinterpret_cast<uint4*>(dst + c + k) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
+        for (int k = 0; k < 32; k++) w[k] = 0;
+      store_rows(stage, w, lane, nq - w_row, dst + c * 128, (int64_t)a.H * (a.nv * 128));
     }
     if (row < nq) a.lse[(int64_t)head * a.Tq + q_lo + row] = live ? (ref + log2f(l)) * 0.693147180559945309f : -INFINITY;
   }
@@ -400,27 +428,6 @@ struct ExBwdArgs {
   DevStatus* st;
 };
 
-// 32 columns of an accumulator, times f, as 32 values of the 16-bit type.
-template <class T>
-LL_DEV void store32(T* dst, const uint32_t* o, float f) {
-#pragma unroll
-  for (int k = 0; k < 32; k += 8) {
-    uint32_t w[4];
-#pragma unroll
-    for (int z = 0; z < 4; z++) w[z] = Num<T>::pack(__uint_as_float(o[k + 2 * z]) * f, __uint_as_float(o[k + 2 * z + 1]) * f);
-    *reinterpret_cast<uint4*>(dst + k) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-LL_DEV void load_acc32(uint32_t at, uint32_t* o, bool any) {
-  if (any) {
-    ld32(at, o);
-    tmem_ld_wait();
-    ld32_ready(o);
-  } else {
-#pragma unroll
-    for (int k = 0; k < 32; k++) o[k] = 0;
-  }
-}
 // Rows from .. rows - 1 of `chunks` consecutive chunks of `rows` rows to zero, by 256 threads.
 LL_DEV void zero_tail(uint8_t* at, int chunks, int rows, int from) {
   for (int i = threadIdx.x; i < (rows - from) * chunks * 8; i += 256) {
@@ -443,6 +450,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
            *sp_full = bars + 7, *sp_free = bars + 8, *ds_ready = bars + 9, *acc_done = bars + 10, *drain = bars + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* s_delta = reinterpret_cast<float*>(tmem_slot + 4);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
 
   if (threadIdx.x == 0) {
@@ -476,25 +484,28 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
-    if (warp == 8 && lane == 0 && n > 0) {
-      // ----------------------------------------------------------------------------- TMA
+    if (warp == 8 && n > 0) {
+      // ----------------------------------------------------------------- TMA (lane c: chunk c)
       bool ok = true;
-      mbar_arrive_expect_tx(q_full, (nqk + a.nv) * kExChunk);
-      for (int c = 0; c < nqk; c++) tma_load_3d(s_q + c * kExChunk, &tm.q, q_full, c * 64, head, q_lo + q0);
-      for (int c = 0; c < a.nv; c++) tma_load_3d(s_g + c * kExChunk, &tm.g, q_full, c * 64, head, q_lo + q0);
+      if (lane == 0) mbar_arrive_expect_tx(q_full, (nqk + a.nv) * kExChunk);
+      __syncwarp();
+      if (lane < nqk) tma_load_3d(s_q + lane * kExChunk, &tm.q, q_full, lane * 64, head, q_lo + q0);
+      else if (lane < nqk + a.nv)
+        tma_load_3d(s_g + (lane - nqk) * kExChunk, &tm.g, q_full, (lane - nqk) * 64, head, q_lo + q0);
       int nk_loads = 0, nv_loads = 0;
       for (int i = 0; i < n && ok; i++) {
+        const int row = k_lo + i * 128;
         if (!(ok = mbar_wait(&k_rel[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.st, 121))) break;
-        mbar_arrive_expect_tx(&k_full[i & 1], nqk * kExChunk);
-        for (int c = 0; c < nqk; c++) {
-          uint8_t* dst = s_k + ((i & 1) * nqk + c) * kExChunk;
-          if (c < a.nn) tma_load_3d(dst, &tm.kn, &k_full[i & 1], c * 64, head, k_lo + i * 128);
-          else tma_load_2d(dst, &tm.kp, &k_full[i & 1], (c - a.nn) * 64, k_lo + i * 128);
-        }
+        if (lane == 0) mbar_arrive_expect_tx(&k_full[i & 1], nqk * kExChunk);
+        __syncwarp();
+        uint8_t* dst = s_k + ((i & 1) * nqk + lane) * kExChunk;
+        if (lane < a.nn) tma_load_3d(dst, &tm.kn, &k_full[i & 1], lane * 64, head, row);
+        else if (lane < nqk) tma_load_2d(dst, &tm.kp, &k_full[i & 1], (lane - a.nn) * 64, row);
         nk_loads++;
         if (!(ok = mbar_wait(v_rel, (i & 1) ^ 1, abort_flag, a.st, 122))) break;
-        mbar_arrive_expect_tx(v_full, a.nv * kExChunk);
-        for (int c = 0; c < a.nv; c++) tma_load_3d(s_v + c * kExChunk, &tm.v, v_full, c * 64, head, k_lo + i * 128);
+        if (lane == 0) mbar_arrive_expect_tx(v_full, a.nv * kExChunk);
+        __syncwarp();
+        if (lane < a.nv) tma_load_3d(s_v + lane * kExChunk, &tm.v, v_full, lane * 64, head, row);
         nv_loads++;
       }
       volatile int keep = 0;                   // everything issued has landed, also after an abort
@@ -507,9 +518,9 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       // ----------------------------------------------------------------------------- MMA
       const bool lead = elect_one();
       const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, 128, false, false);
-      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, 64, false, true);
+      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, nqk * 64, false, true);
       const MmaDesc q_d(smem_u32(s_q), 16, 1024), g_d(smem_u32(s_g), 16, 1024), k_d(smem_u32(s_k), 16, 1024),
-          v_d(smem_u32(s_v), 16, 1024), kt_d(smem_u32(s_k), 1024, 1024);
+          v_d(smem_u32(s_v), 16, 1024), kt_d(smem_u32(s_k), kExChunk, 1024);
       const uint32_t k_tile = nqk * (kExChunk / 16);
       bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag, a.st, 126);
 #pragma unroll 1
@@ -544,12 +555,9 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
         if (!(ok = mbar_wait(ds_ready, i & 1, abort_flag, a.st, 130))) break;
         tc_fence_after();
         if (lead) {
-#pragma unroll 1
-          for (int c = 0; c < nqk; c++)
 #pragma unroll
-            for (int kk = 0; kk < 8; kk++)
-              mma_16bit_ts(tmem + 256 + c * 64, tmem + 448 + kk * 8,
-                           kt_d.lo + (i & 1) * k_tile + c * (kExChunk / 16) + kk * 128, kt_d.hi, id_o, i + kk);
+          for (int kk = 0; kk < 8; kk++)
+            mma_16bit_ts(tmem + 256, tmem + 448 + kk * 8, kt_d.lo + (i & 1) * k_tile + kk * 128, kt_d.hi, id_o, i + kk);
           mma_commit(&k_rel[i & 1]);
           mma_commit(acc_done);
         }
@@ -566,16 +574,33 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const int row = q0 + (warp % 4) * 32 + lane;
     const int see = a.causal ? min(nk, row + nk - nq + 1) : nk, see_all = a.causal ? min(nk, q0 + nk - nq + 1) : nk;
-    float delta = 0.f, lse2 = 0.f;
-    if (row < nq) {
-      const uint4* gp = reinterpret_cast<const uint4*>(static_cast<const T*>(a.g) + (q_lo + row) * a.g_t + head * a.g_h);
-      const uint4* op = reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + ((int64_t)(q_lo + row) * a.H + head) * (a.nv * 64));
-      for (int i = 0; i < a.nv * 8; i++) {
-        const uint4 gv = gp[i], ov = op[i];
-        const T *gx = reinterpret_cast<const T*>(&gv), *ox = reinterpret_cast<const T*>(&ov);
+    {
+      // delta of the tile's rows, sixteen lanes a row and sixteen rows a warp, all loads at once
+      uint4 gv[8], ov[8];
 #pragma unroll
-        for (int z = 0; z < 8; z++) delta = fmaf(Num<T>::to_f(gx[z]), Num<T>::to_f(ox[z]), delta);
+      for (int i = 0; i < 8; i++) {
+        const int r = q0 + warp * 16 + i * 2 + lane / 16, c = lane % 16;
+        gv[i] = ov[i] = make_uint4(0, 0, 0, 0);
+        if (r < nq && c < a.nv * 8) {
+          gv[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.g) + (q_lo + r) * a.g_t + head * a.g_h + c * 8);
+          ov[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + ((int64_t)(q_lo + r) * a.H + head) * (a.nv * 64) + c * 8);
+        }
       }
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const T *gx = reinterpret_cast<const T*>(&gv[i]), *ox = reinterpret_cast<const T*>(&ov[i]);
+        float d = 0.f;
+#pragma unroll
+        for (int z = 0; z < 8; z++) d = fmaf(Num<T>::to_f(gx[z]), Num<T>::to_f(ox[z]), d);
+#pragma unroll
+        for (int off = 8; off; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
+        if (lane % 16 == 0) s_delta[warp * 16 + i * 2 + lane / 16] = d;
+      }
+    }
+    named_bar_sync(1, 256);
+    const float delta = s_delta[row - q0];
+    float lse2 = 0.f;
+    if (row < nq) {
       const int64_t at = (int64_t)head * a.Tq + q_lo + row;
       lse2 = a.lse[at] * 1.4426950408889634f;
       if (cw == 0) a.delta[at] = delta;
@@ -627,11 +652,14 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     }
     if (ok && n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 134);
     tc_fence_after();
-    T* dst = static_cast<T*>(a.dq) + ((int64_t)(q_lo + row) * a.H + head) * (nqk * 64);
-    for (int c = cw * 32; c < nqk * 64; c += 64) {
-      uint32_t o[32];
-      load_acc32(tmem + 256 + lanes + c, o, n > 0);
-      if (row < nq) store32<T>(dst + c, o, a.scale);
+    // every product is done: the query tile (first group) and its gradient's (second) are free as stages
+    const int w_row = row - lane;
+    uint8_t* stage = (cw ? s_g : s_q) + (warp % 4) * 4096;
+    uint8_t* dst = static_cast<uint8_t*>(a.dq) + ((int64_t)(q_lo + w_row) * a.H + head) * (nqk * 128);
+    for (int c = cw; c < nqk; c += 2) {
+      uint32_t w[32];
+      load_acc64<T>(tmem + 256 + lanes + c * 64, n > 0, a.scale, w);
+      store_rows(stage, w, lane, nq - w_row, dst + c * 128, (int64_t)a.H * (nqk * 128));
     }
   }
   tc_fence_before();
@@ -695,23 +723,23 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
-    if (warp == 8 && lane == 0 && n > 0) {
-      // ----------------------------------------------------------------------------- TMA
-      mbar_arrive_expect_tx(kv_full, (nqk + a.nv) * kExChunk);
-      for (int c = 0; c < nqk; c++) {
-        if (c < a.nn) tma_load_3d(s_k + c * kExChunk, &tm.kn, kv_full, c * 64, head, k_lo + k0);
-        else tma_load_2d(s_k + c * kExChunk, &tm.kp, kv_full, (c - a.nn) * 64, k_lo + k0);
-      }
-      for (int c = 0; c < a.nv; c++) tma_load_3d(s_v + c * kExChunk, &tm.v, kv_full, c * 64, head, k_lo + k0);
+    if (warp == 8 && n > 0) {
+      // ----------------------------------------------------------------- TMA (lane c: chunk c)
+      if (lane == 0) mbar_arrive_expect_tx(kv_full, (nqk + a.nv) * kExChunk);
+      __syncwarp();
+      if (lane < a.nn) tma_load_3d(s_k + lane * kExChunk, &tm.kn, kv_full, lane * 64, head, k_lo + k0);
+      else if (lane < nqk) tma_load_2d(s_k + lane * kExChunk, &tm.kp, kv_full, (lane - a.nn) * 64, k_lo + k0);
+      else if (lane < nqk + a.nv)
+        tma_load_3d(s_v + (lane - nqk) * kExChunk, &tm.v, kv_full, (lane - nqk) * 64, head, k_lo + k0);
       int i = 0;
       for (; i < n; i++) {
-        const int s = i % kExQStages;
+        const int s = i % kExQStages, row = q_lo + first + i * kExQ;
         if (!mbar_wait(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 141)) break;
-        mbar_arrive_expect_tx(&q_full[s], stage);
-        const int row = q_lo + first + i * kExQ;
-        for (int c = 0; c < nqk; c++) tma_load_3d(s_qg + s * stage + c * kExQChunk, &tm.q, &q_full[s], c * 64, head, row);
-        for (int c = 0; c < a.nv; c++)
-          tma_load_3d(s_qg + s * stage + (nqk + c) * kExQChunk, &tm.g, &q_full[s], c * 64, head, row);
+        if (lane == 0) mbar_arrive_expect_tx(&q_full[s], stage);
+        __syncwarp();
+        uint8_t* dst = s_qg + s * stage + lane * kExQChunk;
+        if (lane < nqk) tma_load_3d(dst, &tm.q, &q_full[s], lane * 64, head, row);
+        else if (lane < nqk + a.nv) tma_load_3d(dst, &tm.g, &q_full[s], (lane - nqk) * 64, head, row);
       }
       volatile int keep = 0;                   // everything issued has landed, also after an abort
       mbar_wait_sleep(kv_full, 0, &keep, a.st, 142, 64);
@@ -723,9 +751,10 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       // ----------------------------------------------------------------------------- MMA
       const bool lead = elect_one();
       const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, kExQ, false, false);
-      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, 64, false, true);
+      const uint32_t id_k = idesc_16bit(Num<T>::fmt, 128, nqk * 64, false, true);
+      const uint32_t id_v = idesc_16bit(Num<T>::fmt, 128, a.nv * 64, false, true);
       const MmaDesc k_d(smem_u32(s_k), 16, 1024), v_d(smem_u32(s_v), 16, 1024), q_d(smem_u32(s_qg), 16, 1024),
-          qt_d(smem_u32(s_qg), 1024, 1024);
+          qt_d(smem_u32(s_qg), kExQChunk, 1024);
       constexpr uint32_t QC = kExQChunk / 16;
       const uint32_t stage16 = stage / 16;
       bool ok = n == 0 || mbar_wait(kv_full, 0, abort_flag, a.st, 144);
@@ -758,16 +787,12 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
         tc_fence_after();
         if (lead) {
           const uint32_t at = qt_d.lo + (i % kExQStages) * stage16;
-#pragma unroll 1
-          for (int c = 0; c < a.nv; c++)
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-              mma_16bit_ts(tmem + 128 + c * 64, tmem + 448 + kk * 8, at + (nqk + c) * QC + kk * 128, qt_d.hi, id_o, i + kk);
-#pragma unroll 1
-          for (int c = 0; c < nqk; c++)
+          for (int kk = 0; kk < 4; kk++)
+            mma_16bit_ts(tmem + 128, tmem + 448 + kk * 8, at + nqk * QC + kk * 128, qt_d.hi, id_v, i + kk);
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-              mma_16bit_ts(tmem + 256 + c * 64, tmem + 480 + kk * 8, at + c * QC + kk * 128, qt_d.hi, id_o, i + kk);
+          for (int kk = 0; kk < 4; kk++)
+            mma_16bit_ts(tmem + 256, tmem + 480 + kk * 8, at + kk * 128, qt_d.hi, id_k, i + kk);
           mma_commit(&q_rel[i % kExQStages]);
           mma_commit(acc_done);
         }
@@ -848,26 +873,29 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
     }
     if (ok && n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 153);
     tc_fence_after();
-    const int64_t at = (int64_t)(k_lo + row) * a.H + head;
-    for (int c = cw * 32; c < a.nv * 64; c += 64) {
-      uint32_t o[32];
-      load_acc32(tmem + 128 + lanes + c, o, n > 0);
-      if (row < nk) store32<T>(static_cast<T*>(a.dv) + at * (a.nv * 64) + c, o, 1.f);
+    // every product is done: the key tile (first group) and the value tile (second) are free as stages
+    const int w_row = row - lane;
+    uint8_t* stage = (cw ? s_v : s_k) + (warp % 4) * 4096;
+    const int64_t at = (int64_t)(k_lo + w_row) * a.H + head;
+    for (int c = cw; c < a.nv + a.nn; c += 2) {
+      const bool v = c < a.nv;
+      const int cc = v ? c : c - a.nv, chunks = v ? a.nv : a.nn;
+      uint32_t w[32];
+      load_acc64<T>(tmem + lanes + (v ? 128 : 256) + cc * 64, n > 0, v ? 1.f : a.scale, w);
+      store_rows(stage, w, lane, nk - w_row, static_cast<uint8_t*>(v ? a.dv : a.dk) + at * (chunks * 128) + cc * 128,
+                 (int64_t)a.H * (chunks * 128));
     }
-    for (int c = cw * 32; c < nqk * 64; c += 64) {
-      uint32_t o[32];
-      load_acc32(tmem + 256 + lanes + c, o, n > 0);
-      if (row >= nk) continue;
-      if (c < a.nn * 64) {
-        store32<T>(static_cast<T*>(a.dk) + at * (a.nn * 64) + c, o, a.scale);
-      } else {
-        float* dst = a.dkpe + ((int64_t)head * a.Tk + k_lo + row) * (a.nr * 64) + c - a.nn * 64;
-#pragma unroll
-        for (int k = 0; k < 32; k += 4)
-          *reinterpret_cast<float4*>(dst + k) =
-              make_float4(__uint_as_float(o[k]) * a.scale, __uint_as_float(o[k + 1]) * a.scale,
-                          __uint_as_float(o[k + 2]) * a.scale, __uint_as_float(o[k + 3]) * a.scale);
+    for (int c = cw * 32; c < a.nr * 64; c += 64) {
+      uint32_t w[32];
+      if (n > 0) {
+        ld32(tmem + lanes + 256 + a.nn * 64 + c, w);
+        tmem_ld_wait();
+        ld32_ready(w);
       }
+#pragma unroll
+      for (int k = 0; k < 32; k++) w[k] = n > 0 ? __float_as_uint(__uint_as_float(w[k]) * a.scale) : 0u;
+      store_rows(stage, w, lane, nk - w_row,
+                 reinterpret_cast<uint8_t*>(a.dkpe + ((int64_t)head * a.Tk + k_lo + w_row) * (a.nr * 64) + c), a.nr * 256);
     }
   }
   tc_fence_before();
@@ -946,7 +974,7 @@ static int run_backward(const ll_latent_packed* p, const ExTma& tq, const ExTma&
                         cudaStream_t s) {
   const int nqk = a.nn + a.nr;
   if (p->Tq) {
-    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 12 * 8 + 16;
+    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 12 * 8 + 16 + 512;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dq<T>), smem));
     LL_TRY(launch_pdl("k_ex_dq", k_ex_dq<T>, dim3(p->Tq / 128 + p->B, p->H), dim3(kExThreads), smem, s, tq, a));
   }
@@ -984,7 +1012,7 @@ int ll_latent_forward(const ll_latent_packed* p, void* out, float* lse, void* st
   ExFwdArgs a{p->cu_q, p->cu_k, out, lse, p->B, p->Tq, p->Tk, p->H, p->d_n / 64, p->d_r / 64, p->d_v / 64, p->causal,
               p->scale * 1.4426950408889634f, latent_status()};
   if (!a.st) return LL_ERR_CUDA;
-  const int smem = 1024 + (2 * (a.nn + a.nr) + kExRing) * kExChunk + (2 * kExOps + 9) * 8 + 16;
+  const int smem = 1024 + (2 * (a.nn + a.nr) + kExRing) * kExChunk + (2 * kExOps + 11) * 8 + 16;
   auto run = [&](auto kern) {
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(kern), smem));
     return launch_pdl("k_ex_fwd", kern, dim3(p->Tq / 256 + p->B, p->H), dim3(kExThreads), smem, s, tm, a);
