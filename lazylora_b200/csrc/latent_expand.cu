@@ -146,14 +146,15 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
   uint8_t* ring = s_q + 2 * nqk * kExChunk;
   uint64_t* bars = reinterpret_cast<uint64_t*>(ring + kExRing * kExChunk);
   uint64_t *full = bars, *rel = full + kExOps, *q_full = rel + kExOps, *s_full = q_full + 2, *p_ready = s_full + 2,
-           *pv_done = p_ready + 4, *drain = pv_done + 2;
+           *pv_done = p_ready + 2, *drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kExOps + 4; i++) mbar_init(&bars[i], 1);
-    for (int i = 0; i < 4; i++) mbar_init(&p_ready[i], 4);
+    mbar_init(&p_ready[0], 4);
+    mbar_init(&p_ready[1], 4);
     mbar_init(&pv_done[0], 1);
     mbar_init(&pv_done[1], 1);
     mbar_init(drain, 1);
@@ -264,8 +265,6 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
           }
         }
         if (t == 1) {
-          // the key tile is done with; the value tile comes next in the ring
-          if (lead) mma_commit(&rel[(rg.e - 1) % kExOps]);
           if (!(ok = mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 107))) break;
           v_slot = rg.take(a.nv, true);
         }
@@ -273,20 +272,15 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
       const int u = 1 - t, j = i - u;          // the other tile's outputs: O_1(i - 1), O_0(i)
       if (j < 0) continue;
       if (j < (u ? n1 : n0)) {
-#pragma unroll 1
-        for (int half = 0; half < 2; half++) {       // P comes in halves of 64 keys
-          if (!(ok = mbar_wait(&p_ready[2 * u + half], j & 1, abort_flag, a.st, 108))) break;
-          tc_fence_after();
-          if (lead) {
-            const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16) + half * 512;
+        if (!(ok = mbar_wait(&p_ready[u], j & 1, abort_flag, a.st, 108))) break;
+        tc_fence_after();
+        if (lead) {
+          const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16);
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-              mma_16bit_ts(tmem + 256 + u * 128, tmem + u * 128 + half * 32 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o,
-                           j + half + kk);
-          }
+          for (int kk = 0; kk < 8; kk++)
+            mma_16bit_ts(tmem + 256 + u * 128, tmem + u * 128 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o, j + kk);
+          if (j + 1 == (u ? n1 : n0)) mma_commit(&pv_done[u]);
         }
-        if (!ok) break;
-        if (lead) mma_commit(&pv_done[u]);
       }
       if (u == 1 && lead) mma_commit(&rel[(2 * j + 1) % kExOps]);
     }
@@ -311,6 +305,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
       const int v_slot = rv.take(a.nv, true);
       if (!(ok = mbar_wait(&s_full[t], i & 1, abort_flag, a.st, 110))) break;
       tc_fence_after();
+      // the last tile's scores over a key tile release it
+      if (threadIdx.x % 128 == 0 && (t == 1 || i >= n1)) mbar_arrive(&rel[(2 * i) % kExOps]);
       uint32_t x[128];
 #pragma unroll
       for (int c = 0; c < 128; c += 32) ld32(s_at + c, x + c);
@@ -334,8 +330,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
         ref = now;
         l *= f;
         if (i > 0) {
-          if (!(ok = mbar_wait(&pv_done[t], (i - 1) & 1, abort_flag, a.st, 111))) break;
-          tc_fence_after();
+          // (S_t(i) has arrived, and O_t(i - 1) was issued before it: its sums are complete)
           for (int c = 0; c < a.nv * 64; c += 32) {
             uint32_t o[32];
             ld32(o_at + c, o);
@@ -354,7 +349,6 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
         zero_rows(ring, v_slot, a.nv, nk - i * 128, threadIdx.x % 128, 128);
         fence_async_smem();
       }
-      // P in two halves, so that the second one's exponentials run beside the first one's products
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c0 = 0; c0 < 128; c0 += 64) {
@@ -369,14 +363,14 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
           w[c / 2] = Num<T>::pack(u.x, u.y);
         }
         st32(s_at + c0 / 2, w);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[2 * t + c0 / 64]);
       }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_ready[t]);
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
-    if (ok && tiles > 0) ok = mbar_wait(&pv_done[t], (tiles - 1) & 1, abort_flag, a.st, 113);
+    if (ok && tiles > 0) ok = mbar_wait(&pv_done[t], 0, abort_flag, a.st, 113);
     tc_fence_after();
     // the tile's products are done: its first query chunk is free as a stage, 4 KB a warp
     const bool live = !(l <= 0.f);
@@ -1012,7 +1006,7 @@ int ll_latent_forward(const ll_latent_packed* p, void* out, float* lse, void* st
   ExFwdArgs a{p->cu_q, p->cu_k, out, lse, p->B, p->Tq, p->Tk, p->H, p->d_n / 64, p->d_r / 64, p->d_v / 64, p->causal,
               p->scale * 1.4426950408889634f, latent_status()};
   if (!a.st) return LL_ERR_CUDA;
-  const int smem = 1024 + (2 * (a.nn + a.nr) + kExRing) * kExChunk + (2 * kExOps + 11) * 8 + 16;
+  const int smem = 1024 + (2 * (a.nn + a.nr) + kExRing) * kExChunk + (2 * kExOps + 9) * 8 + 16;
   auto run = [&](auto kern) {
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(kern), smem));
     return launch_pdl("k_ex_fwd", kern, dim3(p->Tq / 256 + p->B, p->H), dim3(kExThreads), smem, s, tm, a);
