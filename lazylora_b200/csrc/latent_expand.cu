@@ -13,7 +13,7 @@ namespace ll {
 // tile's softmax runs, the tensor cores do the other's products.
 //   S_t [128][128 keys] = Q_t K^T       (M = 128, N = 128, K = d_n + d_r)
 //   O_t [128][d_v]     += P_t V         (P_t from tensor memory)
-// Issue order per key tile i: S_0(i), O_1(i - 1), S_1(i), O_0(i). Per 256 x 128 scores at 192 / 128 that
+// Issue order per key tile i: O_0(i - 1), S_0(i), O_1(i - 1), S_1(i). Per 256 x 128 scores at 192 / 128 that
 // is 2560 cycles of products against 2048 of exponentials (16 a cycle): the tensor cores bound it.
 // Tensor memory: S_0 | S_1 | O_0 | O_1, 128 columns each; P_t overwrites the first half of S_t.
 //
@@ -241,49 +241,49 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
     bool ok = true;
     ExRing rg;                                 // operands alternate: key tile i is 2 i, value tile 2 i + 1
     int k_slot = 0, v_slot = 0;
+    auto operand = [&]() { return mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 105); };
+    // O_t(i) and S_t(i + 1) in one go, so that nothing is waited for in between
 #pragma unroll 1
-    for (int step = 0; step < 2 * n + 1 && ok; step++) {
-      const int t = step & 1, i = step >> 1;
-      if (i < n) {
-        if (t == 0) {
-          if (!(ok = mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 105))) break;
-          k_slot = rg.take(nqk, false);
-        }
-        if (i < (t ? n1 : n0)) {
-          if (i == 0 && !(ok = mbar_wait(&q_full[t], 0, abort_flag, a.st, 106))) break;
-          tc_fence_after();
-          if (lead) {
-#pragma unroll 1
-            for (int c = 0; c < nqk; c++) {
-              const uint32_t q_lo16 = q_d.lo + (t * nqk + c) * (kExChunk / 16);
-              const uint32_t k_lo16 = k_d.lo + ((k_slot + c) % kExRing) * (kExChunk / 16);
-#pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                mma_16bit(tmem + t * 128, q_lo16 + kk * 2, q_d.hi, k_lo16 + kk * 2, k_d.hi, id_s, c + kk);
-            }
-            mma_commit(&s_full[t]);
-          }
-        }
-        if (t == 1) {
-          if (!(ok = mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 107))) break;
+    for (int step = 0; step < 2 * n + 2 && ok; step++) {
+      const int t = step & 1, i = (step >> 1) - 1, tiles = t ? n1 : n0;
+      if (t == 0) {
+        // value tile i, key tile i + 1
+        if (i >= 0) {
+          if (!(ok = operand())) break;
           v_slot = rg.take(a.nv, true);
         }
-      }
-      const int u = 1 - t, j = i - u;          // the other tile's outputs: O_1(i - 1), O_0(i)
-      if (j < 0) continue;
-      if (j < (u ? n1 : n0)) {
-        if (!(ok = mbar_wait(&p_ready[u], j & 1, abort_flag, a.st, 108))) break;
-        tc_fence_after();
-        if (lead) {
-          const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16);
-#pragma unroll
-          for (int kk = 0; kk < 8; kk++)
-            mma_16bit_ts(tmem + 256 + u * 128, tmem + u * 128 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o, j + kk);
-          if (j + 1 == (u ? n1 : n0)) mma_commit(&pv_done[u]);
+        if (i + 1 < n) {
+          if (!(ok = operand())) break;
+          k_slot = rg.take(nqk, false);
         }
       }
-      if (u == 1 && lead) mma_commit(&rel[(2 * j + 1) % kExOps]);
+      if (i < 0 && tiles > 0 && !(ok = mbar_wait(&q_full[t], 0, abort_flag, a.st, 106))) break;
+      if (i >= 0 && i < tiles) {
+        if (!(ok = mbar_wait(&p_ready[t], i & 1, abort_flag, a.st, 107))) break;
+      }
+      tc_fence_after();
+      if (!lead) continue;
+      if (i >= 0 && i < tiles) {
+        const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16);
+#pragma unroll
+        for (int kk = 0; kk < 8; kk++)
+          mma_16bit_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o, i + kk);
+        if (i + 1 == tiles) mma_commit(&pv_done[t]);
+      }
+      if (i >= 0 && t == 1) mma_commit(&rel[(2 * i + 1) % kExOps]);
+      if (i + 1 < tiles) {
+#pragma unroll 1
+        for (int c = 0; c < nqk; c++) {
+          const uint32_t q_lo16 = q_d.lo + (t * nqk + c) * (kExChunk / 16);
+          const uint32_t k_lo16 = k_d.lo + ((k_slot + c) % kExRing) * (kExChunk / 16);
+#pragma unroll
+          for (int kk = 0; kk < 4; kk++)
+            mma_16bit(tmem + t * 128, q_lo16 + kk * 2, q_d.hi, k_lo16 + kk * 2, k_d.hi, id_s, c + kk);
+        }
+        mma_commit(&s_full[t]);
+      }
     }
+    __syncwarp();
     if (lead) mma_commit(drain);
     volatile int keep = 0;
     mbar_wait_sleep(drain, 0, &keep, a.st, 109, 64);
