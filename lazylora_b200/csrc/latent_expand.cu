@@ -407,8 +407,9 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
 // Tensor memory, 512 columns each:
 //   dq:     S 0 (128), dP 128 (128), dQ 256 (192), dS 448 (64)
 //   dk, dv: S^T 0 (64), dP^T 64 (64), dV 128 (128), dK 256 (192), P^T 448 (32), dS^T 480 (32)
-// Threads: warps 0-3 and 4-7 the element-wise work, each group half of a tile's columns; 8 TMA; 9 MMA; 10
-// (dk, dv) the queries' statistics.
+// Threads: warps 0-3 and 4-7 the element-wise work, each group half of a tile's columns; 8 TMA; 9 the
+// products of S and dP; 11 the sums (a warp that has issued a batch gets on only as the tensor cores take it
+// up, so one issuer alone would leave them idle for its waits); 10 (dk, dv) the queries' statistics.
 struct ExBwdArgs {
   const int32_t *cu_q, *cu_k;
   const void *g, *o;
@@ -442,13 +443,13 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_v + a.nv * kExChunk);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_rel = bars + 3, *v_full = bars + 5, *v_rel = bars + 6,
            *sp_full = bars + 7, *sp_free = bars + 8, *ds_ready = bars + 9, *acc_done = bars + 10, *drain = bars + 11;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_delta = reinterpret_cast<float*>(tmem_slot + 4);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 12; i++) mbar_init(&bars[i], i == 8 || i == 9 ? 8 : 1);
+    for (int i = 0; i < 13; i++) mbar_init(&bars[i], i == 8 || i == 9 ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -512,41 +513,50 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       // ----------------------------------------------------------------------------- MMA
       const bool lead = elect_one();
       const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, 128, false, false);
-      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, nqk * 64, false, true);
       const MmaDesc q_d(smem_u32(s_q), 16, 1024), g_d(smem_u32(s_g), 16, 1024), k_d(smem_u32(s_k), 16, 1024),
-          v_d(smem_u32(s_v), 16, 1024), kt_d(smem_u32(s_k), kExChunk, 1024);
+          v_d(smem_u32(s_v), 16, 1024);
       const uint32_t k_tile = nqk * (kExChunk / 16);
       bool ok = n == 0 || mbar_wait(q_full, 0, abort_flag, a.st, 126);
 #pragma unroll 1
-      for (int i = -1; i < n && ok; i++) {
-        if (i >= 0 && !(ok = mbar_wait(sp_free, i & 1, abort_flag, a.st, 127))) break;
-        const int j = i + 1;
-        if (j < n) {
-          if (!(ok = mbar_wait(&k_full[j & 1], (j >> 1) & 1, abort_flag, a.st, 128))) break;
-          tc_fence_after();
-          if (lead) {
+      for (int j = 0; j < n && ok; j++) {
+        if (j > 0 && !(ok = mbar_wait(sp_free, (j - 1) & 1, abort_flag, a.st, 127))) break;
+        if (!(ok = mbar_wait(&k_full[j & 1], (j >> 1) & 1, abort_flag, a.st, 128))) break;
+        tc_fence_after();
+        if (lead) {
 #pragma unroll 1
-            for (int c = 0; c < nqk; c++)
+          for (int c = 0; c < nqk; c++)
 #pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                mma_16bit(tmem, q_d.lo + c * (kExChunk / 16) + kk * 2, q_d.hi,
-                          k_d.lo + (j & 1) * k_tile + c * (kExChunk / 16) + kk * 2, k_d.hi, id_s, c + kk);
-          }
-          if (!(ok = mbar_wait(v_full, j & 1, abort_flag, a.st, 129))) break;
-          tc_fence_after();
-          if (lead) {
-#pragma unroll 1
-            for (int c = 0; c < a.nv; c++)
-#pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                mma_16bit(tmem + 128, g_d.lo + c * (kExChunk / 16) + kk * 2, g_d.hi, v_d.lo + c * (kExChunk / 16) + kk * 2,
-                          v_d.hi, id_s, c + kk);
-            mma_commit(sp_full);
-            mma_commit(v_rel);
-          }
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit(tmem, q_d.lo + c * (kExChunk / 16) + kk * 2, q_d.hi,
+                        k_d.lo + (j & 1) * k_tile + c * (kExChunk / 16) + kk * 2, k_d.hi, id_s, c + kk);
         }
-        if (i < 0) continue;
-        if (!(ok = mbar_wait(ds_ready, i & 1, abort_flag, a.st, 130))) break;
+        if (!(ok = mbar_wait(v_full, j & 1, abort_flag, a.st, 129))) break;
+        tc_fence_after();
+        if (lead) {
+#pragma unroll 1
+          for (int c = 0; c < a.nv; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit(tmem + 128, g_d.lo + c * (kExChunk / 16) + kk * 2, g_d.hi, v_d.lo + c * (kExChunk / 16) + kk * 2,
+                        v_d.hi, id_s, c + kk);
+          mma_commit(sp_full);
+          mma_commit(v_rel);
+        }
+      }
+      __syncwarp();
+      if (lead) mma_commit(&drain[0]);
+      volatile int keep = 0;
+      mbar_wait_sleep(&drain[0], 0, &keep, a.st, 131, 64);
+      __syncwarp();
+    } else if (warp == 11) {
+      // ------------------------------------------------------------------------ MMA, sums
+      const bool lead = elect_one();
+      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, nqk * 64, false, true);
+      const MmaDesc kt_d(smem_u32(s_k), kExChunk, 1024);
+      const uint32_t k_tile = nqk * (kExChunk / 16);
+#pragma unroll 1
+      for (int i = 0; i < n; i++) {
+        if (!mbar_wait(ds_ready, i & 1, abort_flag, a.st, 130)) break;
         tc_fence_after();
         if (lead) {
 #pragma unroll
@@ -556,9 +566,10 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
           mma_commit(acc_done);
         }
       }
-      if (lead) mma_commit(drain);
+      __syncwarp();
+      if (lead) mma_commit(&drain[1]);
       volatile int keep = 0;
-      mbar_wait_sleep(drain, 0, &keep, a.st, 131, 64);
+      mbar_wait_sleep(&drain[1], 0, &keep, a.st, 135, 64);
       __syncwarp();
     }
   } else {
@@ -679,12 +690,12 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
   uint64_t *kv_full = bars, *q_full = bars + 1, *q_rel = q_full + kExQStages, *st_full = q_rel + kExQStages,
            *sp_full = st_full + kExQStages, *sp_free = sp_full + 1, *ds_ready = sp_full + 2, *acc_done = sp_full + 3,
            *drain = sp_full + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 3 * kExQStages + 6; i++) mbar_init(&bars[i], &bars[i] == sp_free || &bars[i] == ds_ready ? 8 : 1);
+    for (int i = 0; i < 3 * kExQStages + 7; i++) mbar_init(&bars[i], &bars[i] == sp_free || &bars[i] == ds_ready ? 8 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -745,42 +756,49 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       // ----------------------------------------------------------------------------- MMA
       const bool lead = elect_one();
       const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, kExQ, false, false);
-      const uint32_t id_k = idesc_16bit(Num<T>::fmt, 128, nqk * 64, false, true);
-      const uint32_t id_v = idesc_16bit(Num<T>::fmt, 128, a.nv * 64, false, true);
-      const MmaDesc k_d(smem_u32(s_k), 16, 1024), v_d(smem_u32(s_v), 16, 1024), q_d(smem_u32(s_qg), 16, 1024),
-          qt_d(smem_u32(s_qg), kExQChunk, 1024);
+      const MmaDesc k_d(smem_u32(s_k), 16, 1024), v_d(smem_u32(s_v), 16, 1024), q_d(smem_u32(s_qg), 16, 1024);
       constexpr uint32_t QC = kExQChunk / 16;
-      const uint32_t stage16 = stage / 16;
       bool ok = n == 0 || mbar_wait(kv_full, 0, abort_flag, a.st, 144);
 #pragma unroll 1
-      for (int i = -1; i < n && ok; i++) {
-        if (i >= 0 && !(ok = mbar_wait(sp_free, i & 1, abort_flag, a.st, 145))) break;
-        const int j = i + 1;
-        if (j < n) {
-          const int s = j % kExQStages;
-          if (!(ok = mbar_wait(&q_full[s], (j / kExQStages) & 1, abort_flag, a.st, 146))) break;
-          tc_fence_after();
-          if (lead) {
-            const uint32_t at = q_d.lo + s * stage16;
-#pragma unroll 1
-            for (int c = 0; c < nqk; c++)
-#pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                mma_16bit(tmem, k_d.lo + c * (kExChunk / 16) + kk * 2, k_d.hi, at + c * QC + kk * 2, q_d.hi, id_s, c + kk);
-#pragma unroll 1
-            for (int c = 0; c < a.nv; c++)
-#pragma unroll
-              for (int kk = 0; kk < 4; kk++)
-                mma_16bit(tmem + 64, v_d.lo + c * (kExChunk / 16) + kk * 2, v_d.hi, at + (nqk + c) * QC + kk * 2, q_d.hi,
-                          id_s, c + kk);
-            mma_commit(sp_full);
-          }
-        }
-        if (i < 0) continue;
-        if (!(ok = mbar_wait(ds_ready, i & 1, abort_flag, a.st, 147))) break;
+      for (int j = 0; j < n && ok; j++) {
+        const int s = j % kExQStages;
+        if (j > 0 && !(ok = mbar_wait(sp_free, (j - 1) & 1, abort_flag, a.st, 145))) break;
+        if (!(ok = mbar_wait(&q_full[s], (j / kExQStages) & 1, abort_flag, a.st, 146))) break;
         tc_fence_after();
         if (lead) {
-          const uint32_t at = qt_d.lo + (i % kExQStages) * stage16;
+          const uint32_t at = q_d.lo + s * (stage / 16);
+#pragma unroll 1
+          for (int c = 0; c < nqk; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit(tmem, k_d.lo + c * (kExChunk / 16) + kk * 2, k_d.hi, at + c * QC + kk * 2, q_d.hi, id_s, c + kk);
+#pragma unroll 1
+          for (int c = 0; c < a.nv; c++)
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit(tmem + 64, v_d.lo + c * (kExChunk / 16) + kk * 2, v_d.hi, at + (nqk + c) * QC + kk * 2, q_d.hi,
+                        id_s, c + kk);
+          mma_commit(sp_full);
+        }
+      }
+      __syncwarp();
+      if (lead) mma_commit(&drain[0]);
+      volatile int keep = 0;
+      mbar_wait_sleep(&drain[0], 0, &keep, a.st, 148, 64);
+      __syncwarp();
+    } else if (warp == 11) {
+      // ------------------------------------------------------------------------ MMA, sums
+      const bool lead = elect_one();
+      const uint32_t id_k = idesc_16bit(Num<T>::fmt, 128, nqk * 64, false, true);
+      const uint32_t id_v = idesc_16bit(Num<T>::fmt, 128, a.nv * 64, false, true);
+      const MmaDesc qt_d(smem_u32(s_qg), kExQChunk, 1024);
+      constexpr uint32_t QC = kExQChunk / 16;
+#pragma unroll 1
+      for (int i = 0; i < n; i++) {
+        if (!mbar_wait(ds_ready, i & 1, abort_flag, a.st, 147)) break;
+        tc_fence_after();
+        if (lead) {
+          const uint32_t at = qt_d.lo + (i % kExQStages) * (stage / 16);
 #pragma unroll
           for (int kk = 0; kk < 4; kk++)
             mma_16bit_ts(tmem + 128, tmem + 448 + kk * 8, at + nqk * QC + kk * 128, qt_d.hi, id_v, i + kk);
@@ -791,9 +809,10 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
           mma_commit(acc_done);
         }
       }
-      if (lead) mma_commit(drain);
+      __syncwarp();
+      if (lead) mma_commit(&drain[1]);
       volatile int keep = 0;
-      mbar_wait_sleep(drain, 0, &keep, a.st, 148, 64);
+      mbar_wait_sleep(&drain[1], 0, &keep, a.st, 154, 64);
       __syncwarp();
     } else if (warp == 10) {
       // ------------------------------------------------- statistics of the steps' queries
@@ -968,12 +987,12 @@ static int run_backward(const ll_latent_packed* p, const ExTma& tq, const ExTma&
                         cudaStream_t s) {
   const int nqk = a.nn + a.nr;
   if (p->Tq) {
-    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 12 * 8 + 16 + 512;
+    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 13 * 8 + 16 + 512;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dq<T>), smem));
     LL_TRY(launch_pdl("k_ex_dq", k_ex_dq<T>, dim3(p->Tq / 128 + p->B, p->H), dim3(kExThreads), smem, s, tq, a));
   }
   if (p->Tk) {
-    const int smem = 1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 6) * 8 + 16;
+    const int smem = 1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 7) * 8 + 16;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dkv<T>), smem));
     LL_TRY(launch_pdl("k_ex_dkv", k_ex_dkv<T>, dim3(p->Tk / 128 + p->B, p->H), dim3(kExThreads), smem, s, tk, a));
     const int64_t n = (int64_t)p->Tk * p->d_r;

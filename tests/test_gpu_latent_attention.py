@@ -321,6 +321,8 @@ def _expand_exact(q, kn, kp, v, go, out, ql, kl, scale, causal):
     ([70, 260], None, 2, 64, 0, 128, True), ([257], None, 1, 128, 0, 64, False),
     ([600], None, 5, 128, 64, 128, True),
     ([3] * 70 + [200], None, 1, 128, 64, 128, True),              # more sequences than a warp scans at once
+    ([2880, 2305], None, 2, 128, 64, 128, True),                  # long rows of tiles whose last half is empty, or one row
+    ([20, 1], [2500, 1300], 2, 128, 64, 128, True), ([1500], None, 2, 64, 0, 128, False),
 ])
 def test_expanded_forward_and_gradients(dt, ql, kl, H, d_n, d_r, d_v, causal):
     from lazylora_b200.core import latent_attention as A
