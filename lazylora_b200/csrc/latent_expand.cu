@@ -24,9 +24,10 @@ namespace ll {
 // O_t is rescaled only when some row of the warp passes that. P is rounded to the 16-bit type (the tensor
 // cores' operand, the output's own precision); sums in fp32 of the unrounded values.
 constexpr int kExThreads = 384;        // warps 0-3, 4-7: softmax of tile 0, 1; 8: TMA; 9: MMA; 10, 11: none
-// Registers: launched with 168 a thread (64,512 a block); the third warpgroup gives 96 of its up, the two
-// softmax warpgroups take 48 each: 216 * 256 + 72 * 128 = 64,512.
-constexpr int kExRegsMore = 216, kExRegsLess = 72;
+// Registers: launched with 168 a thread (64,512 a block); the third warpgroup gives some of its up to the two
+// softmax warpgroups: 216 * 256 + 72 * 128 = 208 * 256 + 88 * 128 = 64,512. (The backward's issuing warps
+// spill at 72.)
+constexpr int kExRegsMore = 216, kExRegsLess = 72, kExBwdMore = 208, kExBwdLess = 88;
 constexpr int kExRing = 8;
 constexpr int kExChunk = 128 * 128;    // bytes
 constexpr int kExOps = 16;             // barriers of the ring's operands
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
         const bool mine = lane < kExRing && (lane - s0 + kExRing) % kExRing < chunks;
         const int need = __reduce_max_sync(0xffffffffu, mine ? owner : -1);
         if (mine) owner = e;
-        if (need >= 0 && !mbar_wait(&rel[need % kExOps], (need / kExOps) & 1, abort_flag, a.st, 101)) {
+        if (need >= 0 && !mbar_wait_sleep(&rel[need % kExOps], (need / kExOps) & 1, abort_flag, a.st, 101, 64)) {
           rg.e--;
           return false;
         }
@@ -423,6 +424,16 @@ struct ExBwdArgs {
   DevStatus* st;
 };
 
+// P and dS (without the scale) of two scores, in packed operations.
+struct PAndDs {
+  float2 p, ds;
+};
+LL_DEV PAndDs p_and_ds(uint32_t s0, uint32_t s1, uint32_t d0, uint32_t d1, float scale_log2, float2 neg_lse2, float2 neg_delta) {
+  float2 p = fma2(make_float2(__uint_as_float(s0), __uint_as_float(s1)), make_float2(scale_log2, scale_log2), neg_lse2);
+  p.x = ex2(p.x);
+  p.y = ex2(p.y);
+  return {p, mul2(p, add2(make_float2(__uint_as_float(d0), __uint_as_float(d1)), neg_delta))};
+}
 // Rows from .. rows - 1 of `chunks` consecutive chunks of `rows` rows to zero, by 256 threads.
 LL_DEV void zero_tail(uint8_t* at, int chunks, int rows, int from) {
   for (int i = threadIdx.x; i < (rows - from) * chunks * 8; i += 256) {
@@ -478,7 +489,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExBwdLess));
     if (warp == 8 && n > 0) {
       // ----------------------------------------------------------------- TMA (lane c: chunk c)
       bool ok = true;
@@ -490,14 +501,14 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       int nk_loads = 0, nv_loads = 0;
       for (int i = 0; i < n && ok; i++) {
         const int row = k_lo + i * 128;
-        if (!(ok = mbar_wait(&k_rel[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.st, 121))) break;
+        if (!(ok = mbar_wait_sleep(&k_rel[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.st, 121, 64))) break;
         if (lane == 0) mbar_arrive_expect_tx(&k_full[i & 1], nqk * kExChunk);
         __syncwarp();
         uint8_t* dst = s_k + ((i & 1) * nqk + lane) * kExChunk;
         if (lane < a.nn) tma_load_3d(dst, &tm.kn, &k_full[i & 1], lane * 64, head, row);
         else if (lane < nqk) tma_load_2d(dst, &tm.kp, &k_full[i & 1], (lane - a.nn) * 64, row);
         nk_loads++;
-        if (!(ok = mbar_wait(v_rel, (i & 1) ^ 1, abort_flag, a.st, 122))) break;
+        if (!(ok = mbar_wait_sleep(v_rel, (i & 1) ^ 1, abort_flag, a.st, 122, 64))) break;
         if (lane == 0) mbar_arrive_expect_tx(v_full, a.nv * kExChunk);
         __syncwarp();
         if (lane < a.nv) tma_load_3d(s_v + lane * kExChunk, &tm.v, v_full, lane * 64, head, row);
@@ -574,7 +585,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     }
   } else {
     // ---------------------------------------------------------------------- element-wise
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExRegsMore));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExBwdMore));
     const int cw = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const int row = q0 + (warp % 4) * 32 + lane;
@@ -633,19 +644,22 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
         zero_tail(s_k + (i & 1) * nqk * kExChunk, nqk, 128, nk - i * 128);
         fence_async_smem();
       }
-      const bool part = i * 128 + 128 > see_all;
-      const int lim = see - i * 128 - cw * 64;
       uint32_t w[32];
+      if (i * 128 + 128 <= see_all) {          // every row sees every key
 #pragma unroll
-      for (int c = 0; c < 64; c += 2) {
-        float d[2];
-#pragma unroll
-        for (int z = 0; z < 2; z++) {
-          const float p = ex2(fmaf(__uint_as_float(x[c + z]), a.scale_log2, -lse2));
-          d[z] = p * (__uint_as_float(y[c + z]) - delta);
-          if (part && c + z >= lim) d[z] = 0.f;
+        for (int c = 0; c < 64; c += 2) {
+          const float2 d = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(-lse2, -lse2),
+                                    make_float2(-delta, -delta)).ds;
+          w[c / 2] = Num<T>::pack(d.x, d.y);
         }
-        w[c / 2] = Num<T>::pack(d[0], d[1]);
+      } else {
+        const int lim = see - i * 128 - cw * 64;
+#pragma unroll
+        for (int c = 0; c < 64; c += 2) {
+          const float2 d = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(-lse2, -lse2),
+                                    make_float2(-delta, -delta)).ds;
+          w[c / 2] = Num<T>::pack(c < lim ? d.x : 0.f, c + 1 < lim ? d.y : 0.f);
+        }
       }
       if (i > 0 && !(ok = mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 133))) break;
       tc_fence_after();
@@ -685,7 +699,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
   uint8_t* s_k = base;
   uint8_t* s_v = s_k + nqk * kExChunk;
   uint8_t* s_qg = s_v + a.nv * kExChunk;                  // stages of Q and dO
-  float4* s_stat = reinterpret_cast<float4*>(s_qg + kExQStages * stage);      // [stage][32]: (lse, delta) of two queries
+  float4* s_stat = reinterpret_cast<float4*>(s_qg + kExQStages * stage);      // [stage][32]: -lse, -delta of two queries
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_stat + kExQStages * 32);
   uint64_t *kv_full = bars, *q_full = bars + 1, *q_rel = q_full + kExQStages, *st_full = q_rel + kExQStages,
            *sp_full = st_full + kExQStages, *sp_free = sp_full + 1, *ds_ready = sp_full + 2, *acc_done = sp_full + 3,
@@ -727,7 +741,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExBwdLess));
     if (warp == 8 && n > 0) {
       // ----------------------------------------------------------------- TMA (lane c: chunk c)
       if (lane == 0) mbar_arrive_expect_tx(kv_full, (nqk + a.nv) * kExChunk);
@@ -739,7 +753,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       int i = 0;
       for (; i < n; i++) {
         const int s = i % kExQStages, row = q_lo + first + i * kExQ;
-        if (!mbar_wait(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 141)) break;
+        if (!mbar_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 141, 64)) break;
         if (lane == 0) mbar_arrive_expect_tx(&q_full[s], stage);
         __syncwarp();
         uint8_t* dst = s_qg + s * stage + lane * kExQChunk;
@@ -818,15 +832,15 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       // ------------------------------------------------- statistics of the steps' queries
       for (int i = 0; i < n; i++) {
         const int s = i % kExQStages;
-        if (!mbar_wait(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 149)) break;
+        if (!mbar_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 149, 64)) break;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < 2; z++) {
           const int q = first + i * kExQ + lane * 2 + z;
           if (q < nq) {
             const int64_t at = (int64_t)head * a.Tq + q_lo + q;
-            v[2 * z] = a.lse[at] * 1.4426950408889634f;
-            v[2 * z + 1] = a.delta[at];
+            v[z] = -a.lse[at] * 1.4426950408889634f;
+            v[2 + z] = -a.delta[at];
           }
         }
         s_stat[s * 32 + lane] = make_float4(v[0], v[1], v[2], v[3]);
@@ -836,7 +850,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
     }
   } else {
     // ---------------------------------------------------------------------- element-wise
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExRegsMore));
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExBwdMore));
     const int cw = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const int row = k0 + (warp % 4) * 32 + lane;
@@ -859,21 +873,26 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
         zero_tail(s_qg + s * stage, nqk + a.nv, kExQ, nq - qa);
         fence_async_smem();
       }
-      const bool part = qa + kExQ > nq || (a.causal && k0 + 127 > qa + shift);
-      const int from = (a.causal ? row - shift - qa : 0) - cw * 32, to = nq - qa - cw * 32;   // queries that see the row
       uint32_t pw[16], dw[16];
+      const float4* stat = s_stat + s * 32 + cw * 16;
+      if (qa + kExQ <= nq && (!a.causal || k0 + 127 <= qa + shift)) {     // every query sees every row
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        const float4 sd = s_stat[s * 32 + cw * 16 + c / 2];
-        float p[2], d[2];
-#pragma unroll
-        for (int z = 0; z < 2; z++) {
-          p[z] = ex2(fmaf(__uint_as_float(x[c + z]), a.scale_log2, -(z ? sd.z : sd.x)));
-          d[z] = p[z] * (__uint_as_float(y[c + z]) - (z ? sd.w : sd.y));
-          if (part && (c + z < from || c + z >= to)) p[z] = d[z] = 0.f;
+        for (int c = 0; c < 32; c += 2) {
+          const float4 sd = stat[c / 2];
+          const PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y), make_float2(sd.z, sd.w));
+          pw[c / 2] = Num<T>::pack(r.p.x, r.p.y);
+          dw[c / 2] = Num<T>::pack(r.ds.x, r.ds.y);
         }
-        pw[c / 2] = Num<T>::pack(p[0], p[1]);
-        dw[c / 2] = Num<T>::pack(d[0], d[1]);
+      } else {
+        const int from = (a.causal ? row - shift - qa : 0) - cw * 32, to = nq - qa - cw * 32;   // queries that see the row
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const float4 sd = stat[c / 2];
+          const PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y), make_float2(sd.z, sd.w));
+          const bool u = c >= from && c < to, v = c + 1 >= from && c + 1 < to;
+          pw[c / 2] = Num<T>::pack(u ? r.p.x : 0.f, v ? r.p.y : 0.f);
+          dw[c / 2] = Num<T>::pack(u ? r.ds.x : 0.f, v ? r.ds.y : 0.f);
+        }
       }
       if (i > 0 && !(ok = mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 152))) break;
       tc_fence_after();
