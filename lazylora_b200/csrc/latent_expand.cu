@@ -591,16 +591,17 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     const int row = q0 + (warp % 4) * 32 + lane;
     const int see = a.causal ? min(nk, row + nk - nq + 1) : nk, see_all = a.causal ? min(nk, q0 + nk - nq + 1) : nk;
     {
-      // delta of the tile's rows, sixteen lanes a row and sixteen rows a warp, all loads at once
+      // delta of the tile's rows, sixteen lanes a row and sixteen rows a warp, all loads at once (of rows
+      // and columns that exist, whatever is past them: a load under a condition waits for the one before)
+      const int c = min(lane % 16, a.nv * 8 - 1), r0 = q0 + warp * 16 + lane / 16;
+      const T* gp = static_cast<const T*>(a.g) + head * a.g_h + c * 8;
+      const T* op = static_cast<const T*>(a.o) + (int64_t)head * (a.nv * 64) + c * 8;
       uint4 gv[8], ov[8];
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const int r = q0 + warp * 16 + i * 2 + lane / 16, c = lane % 16;
-        gv[i] = ov[i] = make_uint4(0, 0, 0, 0);
-        if (r < nq && c < a.nv * 8) {
-          gv[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.g) + (q_lo + r) * a.g_t + head * a.g_h + c * 8);
-          ov[i] = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o) + ((int64_t)(q_lo + r) * a.H + head) * (a.nv * 64) + c * 8);
-        }
+        const int64_t r = q_lo + max(0, min(r0 + i * 2, nq - 1));
+        gv[i] = *reinterpret_cast<const uint4*>(gp + r * a.g_t);
+        ov[i] = *reinterpret_cast<const uint4*>(op + r * a.H * (a.nv * 64));
       }
 #pragma unroll
       for (int i = 0; i < 8; i++) {
@@ -608,6 +609,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
         float d = 0.f;
 #pragma unroll
         for (int z = 0; z < 8; z++) d = fmaf(Num<T>::to_f(gx[z]), Num<T>::to_f(ox[z]), d);
+        if (lane % 16 >= a.nv * 8) d = 0.f;
 #pragma unroll
         for (int off = 8; off; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
         if (lane % 16 == 0) s_delta[warp * 16 + i * 2 + lane / 16] = d;
