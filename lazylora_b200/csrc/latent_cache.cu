@@ -6,10 +6,11 @@
 // (2i, 2i + 1) or (i, i + d_r / 2). Cosines and sines come from a table row per position: computing
 // them per call would cost more than reading 256 bytes that a token's heads share.
 //
-// Bound by bytes at prompt sizes and by launch latency at a decode step. One block takes a token;
-// an item is 32 bytes in and 32 bytes out (two 16-byte accesses): 16 rotary values of one head (both
-// halves of eight pairs) or 16 latent values, so a token's d_r / 16 (H + 1) + d_c / 16 items share the
-// position's table row through L1. Offsets are 64-bit: a cache passes 2^32 bytes.
+// Bound by bytes at prompt sizes and by launch latency at a decode step. One block takes a token; an item
+// is 16 contiguous bytes in and out: 8 rotary values (pairs side by side), 8 + 8 of two halves (two such
+// pieces), or 8 latent values to copy. A thread requests its first four items before the token's position
+// and its table row (which the heads share through L1) have arrived: three dependent loads become two.
+// Offsets are 64-bit: a cache passes 2^32 bytes.
 #include "latent_ops.cuh"
 
 namespace ll {
@@ -40,80 +41,103 @@ struct AppendArgs {
   void* qo;
   int64_t kv_stride, page_stride, row_stride, q_t, q_h, qo_t, qo_h;
   int64_t n_slots;
-  int table_rows, d_c, d_r, H, page_size, interleaved;
+  int table_rows, d_c, d_r, H, page_size;
+  uint32_t per_inv;  // ceil(2^32 / items of a rotary vector): i / items is the high word of i * per_inv (0: one item)
   float sign;        // -1 turns back
   DevStatus* st;
 };
 
-// Sixteen rotary values of one vector: pairs 8 i .. 8 i + 7.
-template <class T>
-LL_DEV void rotate16(const T* src, T* dst, const float* cs, int d_r, int i, bool interleaved, float sign) {
-  const int h = d_r / 2;
-  const int o0 = interleaved ? 16 * i : 8 * i, o1 = interleaved ? 16 * i + 8 : h + 8 * i;
-  uint4 raw[2] = {*reinterpret_cast<const uint4*>(src + o0), *reinterpret_cast<const uint4*>(src + o1)};
-  float c[8], s[8];
-#pragma unroll
-  for (int j = 0; j < 2; j++) {
-    const float4 cv = *reinterpret_cast<const float4*>(cs + 8 * i + 4 * j);
-    const float4 sv = *reinterpret_cast<const float4*>(cs + h + 8 * i + 4 * j);
-    c[4 * j] = cv.x; c[4 * j + 1] = cv.y; c[4 * j + 2] = cv.z; c[4 * j + 3] = cv.w;
-    s[4 * j] = sign * sv.x; s[4 * j + 1] = sign * sv.y; s[4 * j + 2] = sign * sv.z; s[4 * j + 3] = sign * sv.w;
-  }
-  const T* in = reinterpret_cast<const T*>(raw);
-  float a[8], b[8];
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    a[j] = Num<T>::to_f(in[interleaved ? 2 * j : j]);
-    b[j] = Num<T>::to_f(in[interleaved ? 2 * j + 1 : 8 + j]);
-  }
-  uint32_t w[8];
-#pragma unroll
-  for (int j = 0; j < 8; j++) {
-    const float u = a[j] * c[j] - b[j] * s[j], v = a[j] * s[j] + b[j] * c[j];
-    a[j] = u;
-    b[j] = v;
-  }
-#pragma unroll
-  for (int j = 0; j < 4; j++) {
-    w[j] = interleaved ? Num<T>::pack(a[j], b[j]) : Num<T>::pack(a[2 * j], a[2 * j + 1]);
-    w[4 + j] = interleaved ? Num<T>::pack(a[4 + j], b[4 + j]) : Num<T>::pack(b[2 * j], b[2 * j + 1]);
-  }
-  *reinterpret_cast<uint4*>(dst + o0) = make_uint4(w[0], w[1], w[2], w[3]);
-  *reinterpret_cast<uint4*>(dst + o1) = make_uint4(w[4], w[5], w[6], w[7]);
+// An item's values: one piece of eight (IL: four pairs side by side), or the two pieces that hold the
+// halves of eight pairs.
+template <bool IL>
+struct Piece {
+  uint4 v[IL ? 1 : 2];
+};
+
+template <class T, bool IL>
+LL_DEV Piece<IL> load_piece(const T* src, int d_r, int i) {
+  Piece<IL> p;
+  p.v[0] = *reinterpret_cast<const uint4*>(src + 8 * i);
+  if constexpr (!IL) p.v[1] = *reinterpret_cast<const uint4*>(src + d_r / 2 + 8 * i);
+  return p;
 }
 
-template <class T>
-__global__ void __launch_bounds__(512) k_latent_append(const AppendArgs a) {
-  const int64_t t = blockIdx.x;
-  const int64_t pos = a.positions[t];
-  const bool pos_ok = pos >= 0 && pos < a.table_rows;
-  if (!pos_ok && threadIdx.x == 0) report(a.st, LL_ERR_RANGE, 71, (int)t);
-  const float* cs = a.table + (pos_ok ? pos : 0) * a.d_r;
-  const int per = a.d_r / 16, n_rot = per * a.H;
-  T* row = nullptr;
-  if (a.kv) {
-    const int64_t slot = a.slots[t];
-    if (slot >= a.n_slots && threadIdx.x == 0) report(a.st, LL_ERR_RANGE, 72, (int)t);
-    if (slot >= 0 && slot < a.n_slots && pos_ok)
-      row = static_cast<T*>(a.cache) + (slot / a.page_size) * a.page_stride + (slot % a.page_size) * a.row_stride;
+// Turns item i of a vector by the angles whose cosines, then sines, are at cs.
+template <class T, bool IL>
+LL_DEV void turn_piece(const Piece<IL>& p, T* dst, const float* cs, int d_r, int i, float sign) {
+  constexpr int N = IL ? 4 : 8;
+  const T* in = reinterpret_cast<const T*>(p.v);
+  float a[N], b[N];
+#pragma unroll
+  for (int j = 0; j < N; j += 4) {
+    const float4 c = *reinterpret_cast<const float4*>(cs + N * i + j);
+    const float4 s = *reinterpret_cast<const float4*>(cs + d_r / 2 + N * i + j);
+    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {sign * s.x, sign * s.y, sign * s.z, sign * s.w};
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float x = Num<T>::to_f(in[IL ? 2 * (j + k) : j + k]), y = Num<T>::to_f(in[IL ? 2 * (j + k) + 1 : 8 + j + k]);
+      a[j + k] = x * cc[k] - y * ss[k];
+      b[j + k] = x * ss[k] + y * cc[k];
+    }
   }
-  const int items = n_rot + (a.kv ? per + a.d_c / 16 : 0);
-  for (int i = threadIdx.x; i < items; i += blockDim.x) {
-    if (i < n_rot) {
-      const int h = i / per;
-      if (pos_ok)
-        rotate16<T>(static_cast<const T*>(a.q) + t * a.q_t + h * a.q_h, static_cast<T*>(a.qo) + t * a.qo_t + h * a.qo_h,
-                    cs, a.d_r, i % per, a.interleaved != 0, a.sign);
-    } else if (row) {
-      const T* src = static_cast<const T*>(a.kv) + t * a.kv_stride;
-      const int j = i - n_rot;
-      if (j < per) {
-        rotate16<T>(src + a.d_c, row + a.d_c, cs, a.d_r, j, a.interleaved != 0, a.sign);
-      } else {
-        const int o = (j - per) * 16;
-        const uint4 x = *reinterpret_cast<const uint4*>(src + o), y = *reinterpret_cast<const uint4*>(src + o + 8);
-        *reinterpret_cast<uint4*>(row + o) = x;
-        *reinterpret_cast<uint4*>(row + o + 8) = y;
+  if constexpr (IL) {
+    *reinterpret_cast<uint4*>(dst + 8 * i) =
+        make_uint4(Num<T>::pack(a[0], b[0]), Num<T>::pack(a[1], b[1]), Num<T>::pack(a[2], b[2]), Num<T>::pack(a[3], b[3]));
+  } else {
+    *reinterpret_cast<uint4*>(dst + 8 * i) =
+        make_uint4(Num<T>::pack(a[0], a[1]), Num<T>::pack(a[2], a[3]), Num<T>::pack(a[4], a[5]), Num<T>::pack(a[6], a[7]));
+    *reinterpret_cast<uint4*>(dst + d_r / 2 + 8 * i) =
+        make_uint4(Num<T>::pack(b[0], b[1]), Num<T>::pack(b[2], b[3]), Num<T>::pack(b[4], b[5]), Num<T>::pack(b[6], b[7]));
+  }
+}
+
+constexpr int kAppendThreads = 256, kAppendBatch = 2;
+
+template <class T, bool IL>
+__global__ void __launch_bounds__(kAppendThreads) k_latent_append(const AppendArgs a) {
+  const int64_t t = blockIdx.x;
+  const int per = a.d_r / (IL ? 8 : 16), n_rot = per * a.H, n_new = n_rot + (a.kv ? per : 0);
+  const int items = n_new + (a.kv ? a.d_c / 8 : 0);
+  const T* q = static_cast<const T*>(a.q) + t * a.q_t;
+  const T* kv = static_cast<const T*>(a.kv) + t * a.kv_stride;
+  T* qo = static_cast<T*>(a.qo) + t * a.qo_t;
+  int64_t pos = 0;
+  const float* cs = nullptr;
+  T* row = nullptr;
+  bool known = false;
+  for (int i0 = threadIdx.x; i0 < items; i0 += kAppendThreads * kAppendBatch) {
+    Piece<IL> p[kAppendBatch];
+#pragma unroll
+    for (int u = 0; u < kAppendBatch; u++) {
+      const int i = i0 + u * kAppendThreads;
+      const int h = a.per_inv ? __umulhi(i, a.per_inv) : i;
+      if (i < n_rot) p[u] = load_piece<T, IL>(q + h * a.q_h, a.d_r, i - h * per);
+      else if (i < n_new) p[u] = load_piece<T, IL>(kv + a.d_c, a.d_r, i - n_rot);
+      else if (i < items) p[u].v[0] = *reinterpret_cast<const uint4*>(kv + 8 * (i - n_new));
+    }
+    if (!known) {
+      known = true;
+      pos = a.positions[t];
+      const int64_t slot = a.kv ? a.slots[t] : -1;
+      const bool pos_ok = pos >= 0 && pos < a.table_rows;
+      if (threadIdx.x == 0) {
+        if (!pos_ok) report(a.st, LL_ERR_RANGE, 71, (int)t);
+        if (slot >= a.n_slots) report(a.st, LL_ERR_RANGE, 72, (int)t);
+      }
+      if (!pos_ok) return;
+      cs = a.table + pos * a.d_r;
+      if (slot >= 0 && slot < a.n_slots)
+        row = static_cast<T*>(a.cache) + (slot / a.page_size) * a.page_stride + (slot % a.page_size) * a.row_stride;
+    }
+#pragma unroll
+    for (int u = 0; u < kAppendBatch; u++) {
+      const int i = i0 + u * kAppendThreads;
+      if (i < n_rot) {
+        const int h = a.per_inv ? __umulhi(i, a.per_inv) : i;
+        turn_piece<T, IL>(p[u], qo + h * a.qo_h, cs, a.d_r, i - h * per, a.sign);
+      } else if (row) {
+        if (i < n_new) turn_piece<T, IL>(p[u], row + a.d_c, cs, a.d_r, i - n_rot, a.sign);
+        else if (i < items) *reinterpret_cast<uint4*>(row + 8 * (i - n_new)) = p[u].v[0];
       }
     }
   }
@@ -123,11 +147,11 @@ static bool bad(const void* p, int64_t s0, int64_t s1 = 0) {
   return !p || (reinterpret_cast<uintptr_t>(p) & 15) || s0 % 8 || s1 % 8;
 }
 
-static int launch_append(const AppendArgs& a, int T, int dtype, cudaStream_t s) {
-  const int items = a.d_r / 16 * a.H + (a.kv ? a.d_r / 16 + a.d_c / 16 : 0);
-  const int threads = std::min(512, (items + 31) / 32 * 32);
-  if (dtype == 1) k_latent_append<__nv_bfloat16><<<T, threads, 0, s>>>(a);
-  else k_latent_append<__half><<<T, threads, 0, s>>>(a);
+static int launch_append(AppendArgs& a, int T, int dtype, int interleaved, cudaStream_t s) {
+  if (a.d_r) a.per_inv = (uint32_t)((0xffffffffull + a.d_r / (interleaved ? 8 : 16)) / (a.d_r / (interleaved ? 8 : 16)));
+  auto* fn = dtype == 1 ? (interleaved ? k_latent_append<__nv_bfloat16, true> : k_latent_append<__nv_bfloat16, false>)
+                        : (interleaved ? k_latent_append<__half, true> : k_latent_append<__half, false>);
+  fn<<<T, kAppendThreads, 0, s>>>(a);
   return check_launch("k_latent_append");
 }
 
@@ -164,9 +188,9 @@ int ll_latent_append(const void* kv, int64_t kv_stride, const int64_t* slots, co
   g_launch_count = 0;
   AppendArgs a{kv, slots, positions, table, cache, q_pe, q_out, kv_stride, page_stride, row_stride, q_stride_t,
                q_stride_h, qo_stride_t, qo_stride_h, (int64_t)pages * page_size, table_rows, d_c, d_r, H, page_size,
-               interleaved, 1.f, latent_status()};
+               0, 1.f, latent_status()};
   if (!a.st) return LL_ERR_CUDA;
-  return launch_append(a, T, dtype, s);
+  return launch_append(a, T, dtype, interleaved, s);
 }
 
 int ll_latent_rotate(const void* x, int64_t x_stride_t, int64_t x_stride_h, const int64_t* positions,
@@ -190,11 +214,10 @@ int ll_latent_rotate(const void* x, int64_t x_stride_t, int64_t x_stride_h, cons
   a.qo_h = o_stride_h;
   a.d_r = d_r;
   a.H = H;
-  a.interleaved = interleaved;
   a.sign = inverse ? -1.f : 1.f;
   a.st = latent_status();
   if (!a.st) return LL_ERR_CUDA;
-  return launch_append(a, T, dtype, s);
+  return launch_append(a, T, dtype, interleaved, s);
 }
 
 }  // extern "C"

@@ -60,7 +60,8 @@ def _turn(x, pos, table, interleaved, inverse=False):
 
 @pytest.mark.parametrize("dt", [BF, HF])
 @pytest.mark.parametrize("T,H,d_c,d_r,page,interleaved", [(1, 1, 128, 64, 8, False), (37, 5, 512, 64, 24, True),
-                                                         (130, 64, 256, 32, 48, False), (3, 0, 144, 16, 1, True)])
+                                                         (130, 64, 256, 32, 48, False), (3, 0, 144, 16, 1, True), (9, 7, 128, 16, 8, False),
+                                                         (5, 3, 128, 48, 8, True)])
 def test_append(dt, T, H, d_c, d_r, page, interleaved):
     from lazylora_b200.core import latent_attention as A
     g = _gen(T + H)
