@@ -18,6 +18,7 @@ position, slot or page out of range). Tensors may be strided: the last dimension
 multiples of 8 elements and 16-byte aligned starts; others are copied once.
 """
 import ctypes
+import functools
 from typing import Optional, Tuple
 
 import torch
@@ -38,15 +39,28 @@ def _code(t: torch.Tensor, *others) -> int:
     return _DTYPES[dt]
 
 
+_library = None
+_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _lib():
+    global _library
+    if _library is None:
+        _library = L.load()
+    return _library
+
+
 def _stream(*tensors) -> int:
     """The current stream, for CUDA tensors that all lie on the current device."""
-    dev = torch.cuda.current_device()
+    dev = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
-            if not t.is_cuda:
-                raise ValueError("lazylora_b200 works on CUDA tensors only (no CPU fallback)")
-            raise ValueError(f"a tensor on {t.device}, while the current device is {dev}")
-    return torch._C._cuda_getCurrentRawStream(dev)
+            raise ValueError("latent attention takes tensors of one CUDA device (no CPU fallback)")
+    if dev < 0:
+        raise ValueError("lazylora_b200 works on CUDA tensors only (no CPU fallback)")
+    if dev != _device():
+        raise ValueError(f"tensors on cuda:{dev}, while the current device is another")
+    return _raw_stream(dev)
 
 
 def _view(t: torch.Tensor, copy: bool = True):
@@ -129,7 +143,7 @@ def append_latent(cache: torch.Tensor, kv: torch.Tensor, slots: torch.Tensor, po
         H, os_, qp, op = q_pe.shape[1], ov[1], src.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q_pe")
-    rc = L.load().ll_latent_append(kv.data_ptr(), ks[0], slots.data_ptr(), positions.data_ptr(), table.data_ptr(),
+    rc = _lib().ll_latent_append(kv.data_ptr(), ks[0], slots.data_ptr(), positions.data_ptr(), table.data_ptr(),
                                    table.shape[0], T, d_c, d_r, dt, interleaved, cache.data_ptr(), cs[0], cs[1],
                                    cache.shape[0], cache.shape[1], qp, qs[0], qs[1], H, op, os_[0], os_[1], stream)
     if rc:
@@ -153,12 +167,17 @@ def rotate_positions(x: torch.Tensor, positions: torch.Tensor, table: torch.Tens
     ov = _view(out, copy=False)
     if out.shape != x.shape or ov is None:
         raise ValueError("out: x's shape, contiguous rows, strides multiples of 8, 16-byte aligned")
-    rc = L.load().ll_latent_rotate(src.data_ptr(), xs[0], xs[1], positions.data_ptr(), table.data_ptr(),
+    rc = _lib().ll_latent_rotate(src.data_ptr(), xs[0], xs[1], positions.data_ptr(), table.data_ptr(),
                                    table.shape[0], T, H, d_r, dt, interleaved, inverse, out.data_ptr(), ov[1][0],
                                    ov[1][1], stream)
     if rc:
         L.check(rc, "ll_latent_rotate")
     return out
+
+
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(B: int, Tq: int, H: int, d_c: int) -> int:
+    return _lib().ll_paged_latent_workspace_bytes(B, Tq, H, d_c)
 
 
 def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -191,8 +210,8 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
     out, lse = src.new_empty((B, Tq, H, d_c)), src.new_empty((B, Tq, H), dtype=torch.float32)
     if B == 0 or Tq == 0 or H == 0:
         return out, lse
-    lib, cs = L.load(), cv[1]
-    n = lib.ll_paged_latent_workspace_bytes(B, Tq, H, d_c)
+    lib, cs = _lib(), cv[1]
+    n = _paged_workspace(B, Tq, H, d_c)
     ws = src.new_empty(n, dtype=torch.uint8)
     rc = lib.ll_paged_latent_attention(src.data_ptr(), qs[0], qs[2] if H > 1 else qs[1], cache.data_ptr(), cs[0], cs[1],
                                        pages, page_size, block_table.data_ptr(), block_table.stride(0),
@@ -224,7 +243,7 @@ def head_linear(x: torch.Tensor, w: torch.Tensor, w_nk: bool = True, out: Option
     if out.shape != (T, H, N) or ov is None:
         raise ValueError("out [T, H, N]: contiguous rows, strides multiples of 8, 16-byte aligned")
     os_ = ov[1]
-    rc = L.load().ll_gemm_bf16_heads(T, H, N, K, x.data_ptr(), xs[0], xs[1], w.data_ptr(), ws[0], ws[1], w_nk,
+    rc = _lib().ll_gemm_bf16_heads(T, H, N, K, x.data_ptr(), xs[0], xs[1], w.data_ptr(), ws[0], ws[1], w_nk,
                                      out.data_ptr(), os_[0], os_[1], stream)
     if rc:
         L.check(rc, "ll_gemm_bf16_heads")
@@ -268,7 +287,7 @@ def latent_attention_forward(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Option
     stream = _stream(q, k_nope, k_pe, v, cu_q, cu_k)
     p, keep = _packed(q, k_nope, k_pe, v, cu_q, cu_k, scale, causal)
     out, lse = q.new_empty((p.Tq, p.H, p.d_v)), q.new_empty((p.H, p.Tq), dtype=torch.float32)
-    rc = L.load().ll_latent_forward(ctypes.byref(p), out.data_ptr(), lse.data_ptr(), stream)
+    rc = _lib().ll_latent_forward(ctypes.byref(p), out.data_ptr(), lse.data_ptr(), stream)
     if rc:
         L.check(rc, "ll_latent_forward")
     return out, lse
@@ -286,7 +305,7 @@ def latent_attention_backward(g: torch.Tensor, out: torch.Tensor, lse: torch.Ten
     if g.shape != (Tq, H, d_v) or out.shape != (Tq, H, d_v) or lse.shape != (H, Tq) or lse.dtype is not torch.float32:
         raise ValueError("g and out [Tq, H, d_v], lse fp32 [H, Tq]")
     (g, gs), out, lse = _view(g), _view(out.contiguous())[0], lse.contiguous()
-    lib = L.load()
+    lib = _lib()
     dq, dk, dv = q.new_empty((Tq, H, p.d_n + d_r)), q.new_empty((Tk, H, p.d_n)), q.new_empty((Tk, H, d_v))
     dkpe = q.new_empty((Tk, d_r)) if d_r else None
     n = lib.ll_latent_backward_workspace_bytes(ctypes.byref(p))
