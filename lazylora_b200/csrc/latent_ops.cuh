@@ -49,18 +49,9 @@ LL_DEV bool elect_one() {
   return r != 0;
 }
 
-// Whether a barrier's phase has completed, without the suspension that try_wait may add: for a thread
-// that polls several.
-LL_DEV bool mbar_test(uint64_t* bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.b32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(smem_u32(bar)), "r"(parity)
-      : "memory");
-  return ok != 0;
+// More bytes for the current phase to wait for, without arriving.
+LL_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
 // A shared-memory operand descriptor (128-byte swizzle) as its two words: steps along the operand are

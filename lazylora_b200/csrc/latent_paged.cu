@@ -168,9 +168,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   uint8_t* s_q = s_kv + 2 * tile_bytes;               // [chunk][NT rows][128 bytes]
   uint8_t* s_p = s_q + nchunk * NT * 128;             // [64 keys][128 bytes]: P^T, rows of NT values
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_p + kPgKeys * 128);
-  uint64_t *kv_full = bars, *kv_empty = bars + 2, *s_full = bars + 4, *q_full = bars + 6, *q_empty = bars + 7,
-           *p_ready = bars + 8, *pv_done = bars + 9, *o_free = bars + 10, *drain = bars + 11;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 12);
+  uint64_t *kv_full = bars, *kv_empty = bars + 2, *s_full = bars + 6, *q_full = bars + 8, *q_empty = bars + 9,
+           *p_ready = bars + 10, *o_done = bars + 11, *o_free = bars + 12, *drain = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);        // first sequence, first tile of it, tiles before, after
   float* s_red = reinterpret_cast<float*>(tmem_slot + 8);              // [4 warps][64]
@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   const int g = blockIdx.x / a.RT, rt = blockIdx.x % a.RT;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < 12; i++) mbar_init(&bars[i], i == 8 || i == 10 ? kPgSoft / 32 : 1);
+    for (int i = 0; i < 14; i++) mbar_init(&bars[i], i == 10 || i == 12 ? kPgSoft / 32 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -250,16 +250,20 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
           else report(a.st, LL_ERR_RANGE, 73, w.b);
         }
         const int off = key % a.page_size;
-        if (lane == 0) {
-          ok = mbar_wait(&kv_empty[st], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 81);
-          if (ok) mbar_arrive_expect_tx(&kv_full[st], groups * group_bytes);
-        }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
-        if (!ok) break;
-        if (lane < groups) tma_load_4d(s_kv + st * tile_bytes + lane * group_bytes, &tm.kv, &kv_full[st], 0, off, 0, page);
+        // the second product releases a stage by halves, so the first four groups go ahead
+        if (!(ok = mbar_wait(&kv_empty[st * 2], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 81))) break;
+        if (lane == 0) mbar_expect_tx(&kv_full[st], min(groups, 4) * group_bytes);
+        __syncwarp();
+        uint8_t* dst = s_kv + st * tile_bytes + lane * group_bytes;
+        if (lane < min(groups, 4)) tma_load_4d(dst, &tm.kv, &kv_full[st], 0, off, 0, page);
+        ok = mbar_wait(&kv_empty[st * 2 + 1], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 82);
+        if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], ok ? max(groups - 4, 0) * group_bytes : 0);
+        __syncwarp();
+        if (!ok) { n++; break; }
+        if (lane >= 4 && lane < groups) tma_load_4d(dst, &tm.kv, &kv_full[st], 0, off, 0, page);
         if (j == j0) {
           if (lane == 0) {
-            ok = mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, a.st, 82);
+            ok = mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, a.st, 80);
             if (ok) mbar_arrive_expect_tx(q_full, nchunk * NT * 128);
           }
           ok = __shfl_sync(0xffffffffu, ok, 0);
@@ -276,10 +280,9 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     __syncwarp();
   } else if (warp == 9) {
     // ------------------------------------------------------------------------------- MMA
-    // The whole warp runs the loop (so that descriptors stay in uniform registers), one elected
-    // lane issues. S^T of tile n + 1 goes ahead of tile n's second product when its tile has already
-    // landed, and behind it otherwise: with two tiles in flight, waiting for a tile while a second
-    // product could run would hold up the very stage that the next tile is to land in.
+    // The whole warp runs the loop (so that descriptors stay in uniform registers), one elected lane issues.
+    // Strictly S^T(n), then tile n's second product: issuing S^T(n + 1) in between would hold up the release
+    // of the stage that tile n + 2 lands in, and the loads are what bounds the loop (measured 5 % slower).
     const bool lead = elect_one();
     const uint32_t id_s = idesc_16bit(Num<T>::fmt, 64, NT, false, false);
     const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, NT, true, true);
@@ -287,60 +290,45 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     const MmaDesc k_d(smem_u32(s_kv), 16, group_bytes), v_d(smem_u32(s_kv), 1024, group_bytes);
     const uint32_t tile16 = tile_bytes >> 4, group16 = group_bytes >> 4;
     const int mts = a.nc / 2;
-    uint32_t qk = 0, pv = 0, seg = 0, seg_pv = 0, first_bits = 0;   // first_bits: tile is its piece's first
-    int j = w.j;
-    long long t0 = clock64();
-    while (pv < (uint32_t)count) {
-      bool did = false;
-      if (qk < (uint32_t)count && qk == pv && mbar_test(&kv_full[qk & 1], (qk >> 1) & 1) &&
-          (j != w.j || mbar_test(q_full, seg & 1))) {
+    uint32_t n = 0, piece = 0;
+    bool ok = true;
+    for (; w.left > 0 && ok; w.next(a), piece++) {
+      const int j0 = w.j, j1 = w.end();
+#pragma unroll 1
+      for (int j = j0; j < j1; j++, n++) {
+        const bool first = j == j0;
+        if (!(ok = mbar_wait(&kv_full[n & 1], (n >> 1) & 1, abort_flag, a.st, 86))) break;
+        if (first && !(ok = mbar_wait(q_full, piece & 1, abort_flag, a.st, 87))) break;
         tc_fence_after();
-        const uint32_t at = tmem_s + (qk & 1) * 64, k0 = k_d.lo + (qk & 1) * tile16;
+        const uint32_t at = tmem_s + (n & 1) * 64, k0 = k_d.lo + (n & 1) * tile16, v0 = v_d.lo + (n & 1) * tile16;
         if (lead) {
           for (int c = 0; c < nchunk; c++)
 #pragma unroll
             for (int kk = 0; kk < 4; kk++)
               mma_16bit(at, k0 + c * 64 + kk * 2, k_d.hi, q_d.lo + c * (NT * 8) + kk * 2, q_d.hi, id_s, c + kk);
-          mma_commit(&s_full[qk & 1]);
-          if (j == w.end() - 1) mma_commit(q_empty);
+          mma_commit(&s_full[n & 1]);
+          if (j == j1 - 1) mma_commit(q_empty);
         }
-        first_bits = (first_bits & ~(1u << (qk & 1))) | (j == w.j ? 1u : 0u) << (qk & 1);
-        qk++;
-        if (++j == w.end()) {
-          w.next(a);
-          j = w.j;
-          seg++;
-        }
-        did = true;
-      }
-      const bool first = first_bits >> (pv & 1) & 1;
-      if (pv < qk && mbar_test(p_ready, pv & 1) && (!first || seg_pv == 0 || mbar_test(o_free, (seg_pv - 1) & 1))) {
+        if (!(ok = mbar_wait(p_ready, n & 1, abort_flag, a.st, 88))) break;
+        if (first && piece > 0 && !(ok = mbar_wait(o_free, (piece - 1) & 1, abort_flag, a.st, 89))) break;
         tc_fence_after();
-        const uint32_t v0 = v_d.lo + (pv & 1) * tile16;
         if (lead) {
 #pragma unroll
-          for (int kk = 0; kk < kPgKeys / 16; kk++)
+          for (int half = 0; half < 2; half++) {
 #pragma unroll
-            for (int mt = 0; mt < 4; mt++)
-              if (mt < mts)
-                mma_16bit(tmem + mt * NT, v0 + kk * 2 * group16 + mt * 128, v_d.hi, p_d.lo + kk * 128, p_d.hi, id_o,
-                          first && kk == 0 ? 0 : 1);
-          mma_commit(&kv_empty[pv & 1]);
-          mma_commit(pv_done);
+            for (int kk = half * 2; kk < half * 2 + 2; kk++)
+#pragma unroll
+              for (int mt = 0; mt < 4; mt++)
+                if (mt < mts)
+                  mma_16bit(tmem + mt * NT, v0 + kk * 2 * group16 + mt * 128, v_d.hi, p_d.lo + kk * 128, p_d.hi, id_o,
+                            first && kk == 0 ? 0 : 1);
+            mma_commit(&kv_empty[(n & 1) * 2 + half]);
+          }
+          if (j == j1 - 1) mma_commit(o_done);
         }
-        pv++;
-        // a piece's first tile opens the next piece's wait for its outputs
-        if (first) seg_pv++;
-        did = true;
-      }
-      if (did) t0 = clock64();
-      else if (*abort_flag) break;
-      else if (clock64() - t0 > kWaitLimitCycles) {
-        *abort_flag = 1;
-        if (lead) report(a.st, LL_ERR_TIMEOUT, 86, (int)pv);
-        break;
       }
     }
+    __syncwarp();
     if (lead) mma_commit(drain);
     volatile int keep = 0;
     mbar_wait_sleep(drain, 0, &keep, a.st, 90, 64);
@@ -354,7 +342,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const int t0 = (rt * NT + r0) / a.H, h0 = (rt * NT + r0) % a.H;
     uint8_t* p_row = s_p + (key_in / 8) * 1024 + (key_in % 8) * 128;
-    uint32_t n = 0;
+    uint32_t n = 0, piece = 0;
     for (; w.left > 0; w.next(a)) {
       const int j0 = w.j, j1 = w.end();
       float ref[NQ], l[NQ];
@@ -418,7 +406,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
           v[c] = ex2(v[c]);
           l[c] += v[c];
         }
-        if (n > 0) mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.st, 92);      // P and O are free
+        // (S^T(n) was issued after tile n - 1's second product: P and O are free)
         if (slow && j > j0) {
           tc_fence_after();
           for (int i = side; i < a.nc / 2 * (NT / 16); i += 2) {
@@ -474,7 +462,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         }
       }
       named_bar_sync(1, kPgSoft);
-      mbar_wait(pv_done, (n - 1) & 1, abort_flag, a.st, 93);
+      mbar_wait(o_done, piece & 1, abort_flag, a.st, 93);
+      piece++;
       tc_fence_after();
       const int d_c = a.nc * 64;
       for (int j = side; j < a.nc / 2 * (NT / 16); j += 2) {
@@ -616,7 +605,7 @@ static int launch_paged(const PagedTma& tm, const PagedArgs& a, int smem, cudaSt
 
 template <class T>
 static int run_paged(const PagedTma& tm, const PagedArgs& a, int NT, cudaStream_t s) {
-  const int smem = 1024 + 2 * a.nchunk * 8192 + a.nchunk * NT * 128 + kPgKeys * 128 + 128 + 4 * 384;
+  const int smem = 1024 + 2 * a.nchunk * 8192 + a.nchunk * NT * 128 + kPgKeys * 128 + 144 + 4 * 384;
   if (NT == 16) LL_TRY((launch_paged<T, 16>(tm, a, smem, s)));
   else if (NT == 32) LL_TRY((launch_paged<T, 32>(tm, a, smem, s)));
   else if (NT == 48) LL_TRY((launch_paged<T, 48>(tm, a, smem, s)));
