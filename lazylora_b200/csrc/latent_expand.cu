@@ -482,21 +482,6 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     q0 = 0;
   }
   const int nq = q_hi - q_lo, nk = k_hi - k_lo, n = key_tiles(q0, 128, nq, nk, a.causal);
-  // delta of the tile's rows, sixteen lanes a row and sixteen rows a warp: the loads, all at once and before
-  // the block's set-up is waited for (of rows and columns that exist, whatever is past them: a load under a
-  // condition waits for the one before)
-  uint4 gv[8], ov[8];
-  if (warp < 8) {
-    const int c = min(lane % 16, a.nv * 8 - 1), r0 = q0 + warp * 16 + lane / 16;
-    const T* gp = static_cast<const T*>(a.g) + head * a.g_h + c * 8;
-    const T* op = static_cast<const T*>(a.o) + (int64_t)head * (a.nv * 64) + c * 8;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const int64_t r = q_lo + max(0, min(r0 + i * 2, nq - 1));
-      gv[i] = *reinterpret_cast<const uint4*>(gp + r * a.g_t);
-      ov[i] = *reinterpret_cast<const uint4*>(op + r * a.H * (a.nv * 64));
-    }
-  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -606,6 +591,18 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     const int row = q0 + (warp % 4) * 32 + lane;
     const int see = a.causal ? min(nk, row + nk - nq + 1) : nk, see_all = a.causal ? min(nk, q0 + nk - nq + 1) : nk;
     {
+      // delta of the tile's rows, sixteen lanes a row and sixteen rows a warp, all loads at once (of rows and
+      // columns that exist, whatever is past them: a load under a condition waits for the one before)
+      uint4 gv[8], ov[8];
+      const int c = min(lane % 16, a.nv * 8 - 1), r0 = q0 + warp * 16 + lane / 16;
+      const T* gp = static_cast<const T*>(a.g) + head * a.g_h + c * 8;
+      const T* op = static_cast<const T*>(a.o) + (int64_t)head * (a.nv * 64) + c * 8;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const int64_t r = q_lo + max(0, min(r0 + i * 2, nq - 1));
+        gv[i] = *reinterpret_cast<const uint4*>(gp + r * a.g_t);
+        ov[i] = *reinterpret_cast<const uint4*>(op + r * a.H * (a.nv * 64));
+      }
 #pragma unroll
       for (int i = 0; i < 8; i++) {
         const T *gx = reinterpret_cast<const T*>(&gv[i]), *ox = reinterpret_cast<const T*>(&ov[i]);
