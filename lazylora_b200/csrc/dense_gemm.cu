@@ -24,6 +24,7 @@
 
 #include "host_common.cuh"
 #include "ops.cuh"
+#include "latent_ops.cuh"
 
 namespace ll {
 
@@ -167,7 +168,42 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------------- MMA issuer
-    if (lane == 0) {
+    if (HEADS) {
+      // The whole warp runs the loop, so that the descriptors stay in uniform registers and step by
+      // additions, and one elected lane issues: a narrow tile's 64-cycle products are short against the
+      // 130 cycles an instruction that building each descriptor in one lane takes.
+      const bool lead = elect_one();
+      const DenseJob& jb = args.job[0];
+      const bool bmn = jb.b_mn[0] != 0;
+      const uint32_t idesc = idesc_bf16_m128_major(BN, bmn), b_step = bmn ? 128 : 2;
+      const MmaDesc a_d(smem_u32(stages), 16, 1024), b_d(smem_u32(stages) + kDnAStage, bmn ? 64 * 128 : 16, 1024);
+      int s = 0, ab = 0;
+      uint32_t ph = 0, abph = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; u < args.tiles && ok; u += gridDim.x) {
+        if (!(ok = mbar_wait(&accempty[ab], abph ^ 1, abort_flag, st, 37))) break;
+        tc_fence_after();
+        const uint32_t d = tmem + ab * 256;
+        for (int kb = 0; kb < jb.kb[0]; kb++) {
+          if (!(ok = mbar_wait(&full[s], ph, abort_flag, st, 38))) break;
+          tc_fence_after();
+          const uint32_t at = s * (STG / 16);
+          if (lead) {
+#pragma unroll
+            for (int kk = 0; kk < kDnBK / 16; kk++)
+              mma_16bit(d, a_d.lo + at + kk * 2, a_d.hi, b_d.lo + at + kk * b_step, b_d.hi, idesc, kb + kk);
+            mma_commit(&empty[s]);
+            if (kb + 1 == jb.kb[0]) mma_commit(&accfull[ab]);
+          }
+          if (++s == S) { s = 0; ph ^= 1; }
+        }
+        if (++ab == 2) { ab = 0; abph ^= 1; }
+      }
+      __syncwarp();
+      if (lead) mma_commit(drain);
+      volatile int keep_waiting = 0;
+      mbar_wait_sleep(drain, 0, &keep_waiting, st, 45, 256);
+    } else if (lane == 0) {
       int s = 0, ab = 0;
       uint32_t ev = 0;
       bool ok = true;
@@ -211,7 +247,7 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
     __syncwarp();
   } else if (warp == 6) {
     // ---------------------------------------------------------------------- watcher
-    if (lane == 0) {
+    if (!HEADS && lane == 0) {
       int s = 0, ab = 0;
       uint32_t ph = 0, abph = 0, ev = 0;
       for (int u = blockIdx.x; u < args.tiles; u += gridDim.x) {
@@ -245,6 +281,23 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
       const int row = m0 + q * 32 + lane;
       const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + ab * 256;
       for (int c = 0; c < BN; c += 16) {
+        if (HEADS && c + 64 <= BN && n0 + c + 64 <= args.N) {
+          // 64 columns through shared memory: a head's rows lie a token's stride apart, and 16 bytes a row and
+          // instruction made the output the bound (24 us for 900 tokens and 64 heads)
+          uint32_t o[64], w[32];
+          ld32(tbase + c, o);
+          ld32(tbase + c + 32, o + 32);
+          tmem_ld_wait();
+          ld32_ready(o);
+          ld32_ready(o + 32);
+#pragma unroll
+          for (int i = 0; i < 32; i++) w[i] = Num<__nv_bfloat16>::pack(__uint_as_float(o[2 * i]), __uint_as_float(o[2 * i + 1]));
+          store_rows(stages + S * STG + q * 4096, w, lane, args.M - m0 - q * 32,
+                     reinterpret_cast<uint8_t*>(static_cast<__nv_bfloat16*>(jb.C) + hd * args.c_head +
+                                                (int64_t)(m0 + q * 32) * jb.ldc + n0 + c), jb.ldc * 2);
+          c += 48;
+          continue;
+        }
         float v[16];
         tmem_ld16(tbase + c, v);
         tmem_ld_wait();
@@ -675,7 +728,8 @@ static int head_gemm(int T, int H, int N, int K, const void* x, int64_t x_t, int
   a.BN = pick_bn(T, N, H, !w_nk, di.sms, false);
   a.mt = (T + 127) / 128;
   a.stage_bytes = kDnAStage + a.BN * kDnBK * 2;
-  a.S = std::min(kDnMaxStages, (kDnSmemBudget - 1024 - 1024) / a.stage_bytes);
+  constexpr int kOut = 4 * 4096;               // the epilogue's stage
+  a.S = std::min(kDnMaxStages, (kDnSmemBudget - 1024 - 1024 - kOut) / a.stage_bytes);
   a.n_jobs = 1;
   a.c_bf16 = 1;
   a.c_head = y_h;
@@ -698,7 +752,7 @@ static int head_gemm(int T, int H, int N, int K, const void* x, int64_t x_t, int
   tm.b[1] = tm.b[0];
   a.tiles0 = a.mt * jb.nt;
   a.tiles = a.tiles0 * H;
-  const int smem = 1024 + 1024 + a.S * a.stage_bytes;
+  const int smem = 1024 + 1024 + a.S * a.stage_bytes + kOut;
   LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_dense_gemm<true>), smem));
   const int grid = std::min(a.tiles, di.sms);
   return launch_pdl("k_dense_gemm heads", k_dense_gemm<true>, dim3(grid), dim3(kDnThreads), smem, s, tm, a);

@@ -59,23 +59,6 @@ struct ExRing {
   }
 };
 
-LL_DEV void ld32(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-}
-// After tcgen05.wait::ld: no use of r is scheduled before this point.
-LL_DEV void ld32_ready(uint32_t* r) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 8)
-    asm volatile("" : "+r"(r[i]), "+r"(r[i + 1]), "+r"(r[i + 2]), "+r"(r[i + 3]), "+r"(r[i + 4]), "+r"(r[i + 5]),
-                 "+r"(r[i + 6]), "+r"(r[i + 7])::"memory");
-}
 LL_DEV void st32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
@@ -95,23 +78,6 @@ LL_DEV void zero_rows(uint8_t* ring, int slot, int chunks, int from, int t, int 
   }
 }
 
-// Writes 128 bytes of each of a warp's 32 rows (lane = row, w its 32 words) through 4 KB of shared memory, so
-// that eight lanes write a row's 128 bytes at once: rows apart by a token's stride, written 16 bytes a row
-// and instruction, took 4000 cycles a 128 x 128 tile. rows: how many of the 32 exist; stride in bytes.
-LL_DEV void store_rows(uint8_t* stage, const uint32_t* w, int lane, int rows, uint8_t* dst, int64_t stride) {
-#pragma unroll
-  for (int c = 0; c < 8; c++)
-    *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) * 16)) =
-        make_uint4(w[4 * c], w[4 * c + 1], w[4 * c + 2], w[4 * c + 3]);
-  __syncwarp();
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const int r = i * 4 + lane / 8, c = lane % 8;
-    const uint4 v = *reinterpret_cast<const uint4*>(stage + r * 128 + ((c ^ (r & 7)) * 16));
-    if (r < rows) *reinterpret_cast<uint4*>(dst + r * stride + c * 16) = v;
-  }
-  __syncwarp();
-}
 // 64 columns of an accumulator (zeros where nothing was summed), times f, as 32 words of the 16-bit type.
 template <class T>
 LL_DEV void load_acc64(uint32_t at, bool any, float f, uint32_t* w) {
