@@ -32,6 +32,23 @@ constexpr int kExRing = 8;
 constexpr int kExChunk = 128 * 128;    // bytes
 constexpr int kExOps = 16;             // barriers of the ring's operands
 constexpr float kExSlack = 8.f;
+// A wait that runs out records itself and raises the block's abort flag, after which every wait returns at
+// once. The loading warps then stop (all lanes together), the issuing warps too; the element-wise warps go
+// through their loops without leaving them, so that no warp-wide instruction loses lanes; the results are
+// void, as the status says.
+
+// The order in which blocks take (tile, head): heads in groups, in a group the longest tiles of its heads
+// first, so that the launch ends on a group's short tiles; the groups (about four tiles per SM) keep the keys
+// and values in use few enough for L2. A head after the other, the last heads' long tiles ended 12 % after
+// the average SM (8000 tokens, 32 heads: 609 us; groups of 2, 4, 8 tiles an SM: 636, 555, 565).
+struct ExOrder {
+  int tiles, heads, group;
+};
+LL_DEV void ex_deal(const ExOrder& o, int& tile, int& head) {
+  const int per = o.group * o.tiles, g = blockIdx.x / per, r = blockIdx.x % per, n = min(o.group, o.heads - g * o.group);
+  tile = r / n;
+  head = g * o.group + r % n;
+}
 
 struct ExTma {
   CUtensorMap q, kn, kp, v, g;
@@ -42,6 +59,7 @@ struct ExFwdArgs {
   void* out;
   float* lse;
   int B, Tq, Tk, H, nn, nr, nv, causal;    // 64-column chunks of d_n, d_r, d_v
+  ExOrder order;
   float scale_log2;
   DevStatus* st;
 };
@@ -116,7 +134,9 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
            *pv_done = p_ready + 2, *drain = pv_done + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int tile, head;
+  ex_deal(a.order, tile, head);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2 * kExOps + 4; i++) mbar_init(&bars[i], 1);
@@ -138,7 +158,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
   __syncwarp();
   pdl_wait();
   int b, q0, q_lo, q_hi, k_lo, k_hi;
-  const bool any = find_tile<true>(a.cu_q, a.B, a.Tq, 256, blockIdx.x, b, q0);
+  const bool any = find_tile<true>(a.cu_q, a.B, a.Tq, 256, tile, b, q0);
   if (any) {
     seq_range(a.cu_q, b, a.Tq, q_lo, q_hi);
     seq_range(a.cu_k, b, a.Tk, k_lo, k_hi);
@@ -154,123 +174,123 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
   const uint32_t tmem = *tmem_slot;
 
   if (warp >= 8) {
-   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
-   if (warp == 8) {
-    // ------------------------------------------------------------------------------- TMA
-    // Lane c brings chunk c: boxes that one thread issues follow each other about 350 cycles apart.
-    if (n > 0) {
-      ExRing rg;
-      bool ok = true;
-      int owner = -1;                          // lane s: the operand that last took slot s
-      auto load = [&](bool key, int row) {
-        const int chunks = key ? nqk : a.nv, e = rg.e, s0 = rg.take(chunks, !key);
-        const bool mine = lane < kExRing && (lane - s0 + kExRing) % kExRing < chunks;
-        const int need = __reduce_max_sync(0xffffffffu, mine ? owner : -1);
-        if (mine) owner = e;
-        if (need >= 0 && !mbar_wait_sleep(&rel[need % kExOps], (need / kExOps) & 1, abort_flag, a.st, 101, 64)) {
-          rg.e--;
-          return false;
-        }
-        uint64_t* bar = &full[e % kExOps];
-        if (lane == 0) mbar_arrive_expect_tx(bar, chunks * kExChunk);
-        __syncwarp();
-        uint8_t* dst = ring + ((s0 + lane) % kExRing) * kExChunk;
-        if (key && lane < a.nn) tma_load_3d(dst, &tm.kn, bar, lane * 64, head, row);
-        else if (key && lane < nqk) tma_load_2d(dst, &tm.kp, bar, (lane - a.nn) * 64, row);
-        else if (!key && lane < a.nv) tma_load_3d(dst, &tm.v, bar, lane * 64, head, row);
-        __syncwarp();
-        return true;
-      };
-      for (int t = 0; t < 2; t++) {
-        if ((t ? n1 : n0) > 0) {
-          if (lane == 0) mbar_arrive_expect_tx(&q_full[t], nqk * kExChunk);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kExRegsLess));
+    if (warp == 8) {
+      // ------------------------------------------------------------------------------- TMA
+      // Lane c brings chunk c: boxes that one thread issues follow each other about 350 cycles apart.
+      if (n > 0) {
+        ExRing rg;
+        bool ok = true;
+        int owner = -1;                          // lane s: the operand that last took slot s
+        auto load = [&](bool key, int row) {
+          const int chunks = key ? nqk : a.nv, e = rg.e, s0 = rg.take(chunks, !key);
+          const bool mine = lane < kExRing && (lane - s0 + kExRing) % kExRing < chunks;
+          const int need = __reduce_max_sync(0xffffffffu, mine ? owner : -1);
+          if (mine) owner = e;
+          if (need >= 0 && !warp_wait_sleep(&rel[need % kExOps], (need / kExOps) & 1, abort_flag, a.st, 101, 64)) {
+            rg.e--;
+            return false;
+          }
+          uint64_t* bar = &full[e % kExOps];
+          if (lane == 0) mbar_arrive_expect_tx(bar, chunks * kExChunk);
           __syncwarp();
-          if (lane < nqk)
-            tma_load_3d(s_q + (t * nqk + lane) * kExChunk, &tm.q, &q_full[t], lane * 64, head, q_lo + q0 + t * 128);
+          uint8_t* dst = ring + ((s0 + lane) % kExRing) * kExChunk;
+          if (key && lane < a.nn) tma_load_3d(dst, &tm.kn, bar, lane * 64, head, row);
+          else if (key && lane < nqk) tma_load_2d(dst, &tm.kp, bar, (lane - a.nn) * 64, row);
+          else if (!key && lane < a.nv) tma_load_3d(dst, &tm.v, bar, lane * 64, head, row);
+          __syncwarp();
+          return true;
+        };
+        for (int t = 0; t < 2; t++) {
+          if ((t ? n1 : n0) > 0) {
+            if (lane == 0) mbar_arrive_expect_tx(&q_full[t], nqk * kExChunk);
+            __syncwarp();
+            if (lane < nqk)
+              tma_load_3d(s_q + (t * nqk + lane) * kExChunk, &tm.q, &q_full[t], lane * 64, head, q_lo + q0 + t * 128);
+          }
+          if (t == 0) ok = load(true, k_lo);
         }
-        if (t == 0) ok = load(true, k_lo);
+        if (ok) ok = load(false, k_lo);
+        for (int i = 1; i < n && ok; i++) ok = load(true, k_lo + i * 128) && load(false, k_lo + i * 128);
+        volatile int keep = 0;                   // everything issued has landed, also after an abort
+        for (uint32_t e = rg.e > kExRing ? rg.e - kExRing : 0; e < rg.e; e++)
+          mbar_wait_sleep(&full[e % kExOps], (e / kExOps) & 1, &keep, a.st, 102, 64);
+        if (n0 > 0) mbar_wait_sleep(&q_full[0], 0, &keep, a.st, 103, 64);
+        if (n1 > 0) mbar_wait_sleep(&q_full[1], 0, &keep, a.st, 104, 64);
       }
-      if (ok) ok = load(false, k_lo);
-      for (int i = 1; i < n && ok; i++) ok = load(true, k_lo + i * 128) && load(false, k_lo + i * 128);
-      volatile int keep = 0;                   // everything issued has landed, also after an abort
-      for (uint32_t e = rg.e > kExRing ? rg.e - kExRing : 0; e < rg.e; e++)
-        mbar_wait_sleep(&full[e % kExOps], (e / kExOps) & 1, &keep, a.st, 102, 64);
-      if (n0 > 0) mbar_wait_sleep(&q_full[0], 0, &keep, a.st, 103, 64);
-      if (n1 > 0) mbar_wait_sleep(&q_full[1], 0, &keep, a.st, 104, 64);
-    }
-    __syncwarp();
-  } else if (warp == 9) {
-    // ------------------------------------------------------------------------------- MMA
-    const bool lead = elect_one();
-    const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, 128, false, false);
-    const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, a.nv * 64, false, true);
-    const MmaDesc q_d(smem_u32(s_q), 16, 1024), k_d(smem_u32(ring), 16, 1024), v_d(smem_u32(ring), kExChunk, 1024);
-    bool ok = true;
-    ExRing rg;                                 // operands alternate: key tile i is 2 i, value tile 2 i + 1
-    int k_slot = 0, v_slot = 0;
-    auto operand = [&]() { return mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 105); };
-    // O_t(i) and S_t(i + 1) in one go, so that nothing is waited for in between
+      __syncwarp();
+    } else if (warp == 9) {
+      // ------------------------------------------------------------------------------- MMA
+      const bool lead = elect_one();
+      const uint32_t id_s = idesc_16bit(Num<T>::fmt, 128, 128, false, false);
+      const uint32_t id_o = idesc_16bit(Num<T>::fmt, 128, a.nv * 64, false, true);
+      const MmaDesc q_d(smem_u32(s_q), 16, 1024), k_d(smem_u32(ring), 16, 1024), v_d(smem_u32(ring), kExChunk, 1024);
+      bool ok = true;
+      ExRing rg;                                 // operands alternate: key tile i is 2 i, value tile 2 i + 1
+      int k_slot = 0, v_slot = 0;
+      auto operand = [&]() { return mbar_wait(&full[rg.e % kExOps], (rg.e / kExOps) & 1, abort_flag, a.st, 105); };
+      // O_t(i) and S_t(i + 1) in one go, so that nothing is waited for in between
 #pragma unroll 1
-    for (int step = 0; step < 2 * n + 2 && ok; step++) {
-      const int t = step & 1, i = (step >> 1) - 1, tiles = t ? n1 : n0;
-      if (t == 0) {
-        // value tile i, key tile i + 1
-        if (i >= 0) {
-          if (!(ok = operand())) break;
-          v_slot = rg.take(a.nv, true);
+      for (int step = 0; step < 2 * n + 2 && ok; step++) {
+        const int t = step & 1, i = (step >> 1) - 1, tiles = t ? n1 : n0;
+        if (t == 0) {
+          // value tile i, key tile i + 1
+          if (i >= 0) {
+            if (!(ok = operand())) break;
+            v_slot = rg.take(a.nv, true);
+          }
+          if (i + 1 < n) {
+            if (!(ok = operand())) break;
+            k_slot = rg.take(nqk, false);
+          }
         }
-        if (i + 1 < n) {
-          if (!(ok = operand())) break;
-          k_slot = rg.take(nqk, false);
+        if (i < 0 && tiles > 0 && !(ok = mbar_wait(&q_full[t], 0, abort_flag, a.st, 106))) break;
+        if (i >= 0 && i < tiles) {
+          if (!(ok = mbar_wait(&p_ready[t], i & 1, abort_flag, a.st, 107))) break;
         }
-      }
-      if (i < 0 && tiles > 0 && !(ok = mbar_wait(&q_full[t], 0, abort_flag, a.st, 106))) break;
-      if (i >= 0 && i < tiles) {
-        if (!(ok = mbar_wait(&p_ready[t], i & 1, abort_flag, a.st, 107))) break;
-      }
-      tc_fence_after();
-      if (!lead) continue;
-      if (i >= 0 && i < tiles) {
-        const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16);
+        tc_fence_after();
+        if (!lead) continue;
+        if (i >= 0 && i < tiles) {
+          const uint32_t v_lo16 = v_d.lo + v_slot * (kExChunk / 16);
 #pragma unroll
-        for (int kk = 0; kk < 8; kk++)
-          mma_16bit_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o, i + kk);
-        if (i + 1 == tiles) mma_commit(&pv_done[t]);
-      }
-      if (i >= 0 && t == 1) mma_commit(&rel[(2 * i + 1) % kExOps]);
-      if (i + 1 < tiles) {
+          for (int kk = 0; kk < 8; kk++)
+            mma_16bit_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, v_lo16 + kk * 128, v_d.hi, id_o, i + kk);
+          if (i + 1 == tiles) mma_commit(&pv_done[t]);
+        }
+        if (i >= 0 && t == 1) mma_commit(&rel[(2 * i + 1) % kExOps]);
+        if (i + 1 < tiles) {
 #pragma unroll 1
-        for (int c = 0; c < nqk; c++) {
-          const uint32_t q_lo16 = q_d.lo + (t * nqk + c) * (kExChunk / 16);
-          const uint32_t k_lo16 = k_d.lo + ((k_slot + c) % kExRing) * (kExChunk / 16);
+          for (int c = 0; c < nqk; c++) {
+            const uint32_t q_lo16 = q_d.lo + (t * nqk + c) * (kExChunk / 16);
+            const uint32_t k_lo16 = k_d.lo + ((k_slot + c) % kExRing) * (kExChunk / 16);
 #pragma unroll
-          for (int kk = 0; kk < 4; kk++)
-            mma_16bit(tmem + t * 128, q_lo16 + kk * 2, q_d.hi, k_lo16 + kk * 2, k_d.hi, id_s, c + kk);
+            for (int kk = 0; kk < 4; kk++)
+              mma_16bit(tmem + t * 128, q_lo16 + kk * 2, q_d.hi, k_lo16 + kk * 2, k_d.hi, id_s, c + kk);
+          }
+          mma_commit(&s_full[t]);
         }
-        mma_commit(&s_full[t]);
       }
+      __syncwarp();
+      if (lead) mma_commit(drain);
+      volatile int keep = 0;
+      mbar_wait_sleep(drain, 0, &keep, a.st, 109, 64);
+      __syncwarp();
     }
-    __syncwarp();
-    if (lead) mma_commit(drain);
-    volatile int keep = 0;
-    mbar_wait_sleep(drain, 0, &keep, a.st, 109, 64);
-    __syncwarp();
-   }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExRegsMore));
     // --------------------------------------------------------------------------- softmax
     const int t = warp / 4, tiles = t ? n1 : n0;
-    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16, s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
+    const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
+    const uint32_t s_at = tmem + t * 128 + lanes, o_at = tmem + 256 + t * 128 + lanes;
     const int row = q0 + t * 128 + (warp % 4) * 32 + lane;        // of the sequence
     const int see = a.causal ? min(nk, row + nk - nq + 1) : nk;   // keys the row sees
     const int see_all = a.causal ? min(nk, q0 + t * 128 + nk - nq + 1) : nk;   // and the tile's first row
     float ref = -1e30f, l = 0.f;
-    bool ok = true;
     ExRing rv;
     for (int i = 0; i < tiles; i++) {
       rv.take(nqk, false);
       const int v_slot = rv.take(a.nv, true);
-      if (!(ok = mbar_wait(&s_full[t], i & 1, abort_flag, a.st, 110))) break;
+      mbar_wait(&s_full[t], i & 1, abort_flag, a.st, 110);
       tc_fence_after();
       // the last tile's scores over a key tile release it
       if (threadIdx.x % 128 == 0 && (t == 1 || i >= n1)) mbar_arrive(&rel[(2 * i) % kExOps]);
@@ -312,7 +332,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
       if (i * 128 + 128 > nk) {
         // the value rows past the sequence's end, which may hold anything, must not meet P's zeros
         const uint32_t e = 2 * i + 1;
-        if (!(ok = mbar_wait(&full[e % kExOps], (e / kExOps) & 1, abort_flag, a.st, 112))) break;
+        mbar_wait(&full[e % kExOps], (e / kExOps) & 1, abort_flag, a.st, 112);
         zero_rows(ring, v_slot, a.nv, nk - i * 128, threadIdx.x % 128, 128);
         fence_async_smem();
       }
@@ -337,7 +357,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
       if (lane == 0) mbar_arrive(&p_ready[t]);
       l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
-    if (ok && tiles > 0) ok = mbar_wait(&pv_done[t], 0, abort_flag, a.st, 113);
+    if (tiles > 0) mbar_wait(&pv_done[t], 0, abort_flag, a.st, 113);
     tc_fence_after();
     // the tile's products are done: its first query chunk is free as a stage, 4 KB a warp
     const bool live = !(l <= 0.f);
@@ -386,6 +406,7 @@ struct ExBwdArgs {
   float* dkpe;             // [H][Tk][64 nr]
   void *dq, *dk, *dv;
   int B, Tq, Tk, H, nn, nr, nv, causal;
+  ExOrder order;
   float scale, scale_log2;
   DevStatus* st;
 };
@@ -394,7 +415,8 @@ struct ExBwdArgs {
 struct PAndDs {
   float2 p, ds;
 };
-LL_DEV PAndDs p_and_ds(uint32_t s0, uint32_t s1, uint32_t d0, uint32_t d1, float scale_log2, float2 neg_lse2, float2 neg_delta) {
+LL_DEV PAndDs p_and_ds(uint32_t s0, uint32_t s1, uint32_t d0, uint32_t d1, float scale_log2, float2 neg_lse2,
+                       float2 neg_delta) {
   float2 p = fma2(make_float2(__uint_as_float(s0), __uint_as_float(s1)), make_float2(scale_log2, scale_log2), neg_lse2);
   p.x = ex2(p.x);
   p.y = ex2(p.y);
@@ -423,7 +445,9 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* s_delta = reinterpret_cast<float*>(tmem_slot + 4);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int tile, head;
+  ex_deal(a.order, tile, head);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 13; i++) mbar_init(&bars[i], i == 8 || i == 9 ? 8 : 1);
@@ -441,7 +465,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
   __syncwarp();
   pdl_wait();
   int b, q0, q_lo = 0, q_hi = 0, k_lo = 0, k_hi = 0;
-  if (find_tile<true>(a.cu_q, a.B, a.Tq, 128, blockIdx.x, b, q0)) {
+  if (find_tile<true>(a.cu_q, a.B, a.Tq, 128, tile, b, q0)) {
     seq_range(a.cu_q, b, a.Tq, q_lo, q_hi);
     seq_range(a.cu_k, b, a.Tk, k_lo, k_hi);
   } else {
@@ -467,14 +491,14 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       int nk_loads = 0, nv_loads = 0;
       for (int i = 0; i < n && ok; i++) {
         const int row = k_lo + i * 128;
-        if (!(ok = mbar_wait_sleep(&k_rel[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.st, 121, 64))) break;
+        if (!(ok = warp_wait_sleep(&k_rel[i & 1], ((i >> 1) & 1) ^ 1, abort_flag, a.st, 121, 64))) break;
         if (lane == 0) mbar_arrive_expect_tx(&k_full[i & 1], nqk * kExChunk);
         __syncwarp();
         uint8_t* dst = s_k + ((i & 1) * nqk + lane) * kExChunk;
         if (lane < a.nn) tma_load_3d(dst, &tm.kn, &k_full[i & 1], lane * 64, head, row);
         else if (lane < nqk) tma_load_2d(dst, &tm.kp, &k_full[i & 1], (lane - a.nn) * 64, row);
         nk_loads++;
-        if (!(ok = mbar_wait_sleep(v_rel, (i & 1) ^ 1, abort_flag, a.st, 122, 64))) break;
+        if (!(ok = warp_wait_sleep(v_rel, (i & 1) ^ 1, abort_flag, a.st, 122, 64))) break;
         if (lane == 0) mbar_arrive_expect_tx(v_full, a.nv * kExChunk);
         __syncwarp();
         if (lane < a.nv) tma_load_3d(s_v + lane * kExChunk, &tm.v, v_full, lane * 64, head, row);
@@ -482,7 +506,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       }
       volatile int keep = 0;                   // everything issued has landed, also after an abort
       mbar_wait_sleep(q_full, 0, &keep, a.st, 123, 64);
-      for (int i = max(0, nk_loads - 2); i < nk_loads; i++) mbar_wait_sleep(&k_full[i & 1], (i >> 1) & 1, &keep, a.st, 124, 64);
+      for (int i = max(0, nk_loads - 2); i < nk_loads; i++)
+        mbar_wait_sleep(&k_full[i & 1], (i >> 1) & 1, &keep, a.st, 124, 64);
       if (nv_loads > 0) mbar_wait_sleep(v_full, (nv_loads - 1) & 1, &keep, a.st, 125, 64);
     }
     __syncwarp();
@@ -589,9 +614,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       lse2 = a.lse[at] * 1.4426950408889634f;
       if (cw == 0) a.delta[at] = delta;
     }
-    bool ok = true;
     for (int i = 0; i < n; i++) {
-      if (!(ok = mbar_wait(sp_full, i & 1, abort_flag, a.st, 132))) break;
+      mbar_wait(sp_full, i & 1, abort_flag, a.st, 132);
       tc_fence_after();
       uint32_t x[64], y[64];
 #pragma unroll
@@ -629,7 +653,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
           w[c / 2] = Num<T>::pack(c < lim ? d.x : 0.f, c + 1 < lim ? d.y : 0.f);
         }
       }
-      if (i > 0 && !(ok = mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 133))) break;
+      if (i > 0) mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 133);
       tc_fence_after();
       st32(tmem + 448 + lanes + cw * 32, w);
       tmem_st_wait();
@@ -637,7 +661,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
     }
-    if (ok && n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 134);
+    if (n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 134);
     tc_fence_after();
     // every product is done: the query tile (first group) and its gradient's (second) are free as stages
     const int w_row = row - lane;
@@ -674,7 +698,9 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
            *drain = sp_full + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, head = blockIdx.y;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  int tile, head;
+  ex_deal(a.order, tile, head);
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3 * kExQStages + 7; i++) mbar_init(&bars[i], &bars[i] == sp_free || &bars[i] == ds_ready ? 8 : 1);
@@ -692,7 +718,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
   __syncwarp();
   pdl_wait();
   int b, k0, q_lo = 0, q_hi = 0, k_lo = 0, k_hi = 0;
-  if (find_tile<false>(a.cu_k, a.B, a.Tk, 128, blockIdx.x, b, k0)) {
+  if (find_tile<false>(a.cu_k, a.B, a.Tk, 128, tile, b, k0)) {
     seq_range(a.cu_q, b, a.Tq, q_lo, q_hi);
     seq_range(a.cu_k, b, a.Tk, k_lo, k_hi);
   } else {
@@ -721,7 +747,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       int i = 0;
       for (; i < n; i++) {
         const int s = i % kExQStages, row = q_lo + first + i * kExQ;
-        if (!mbar_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 141, 64)) break;
+        if (!warp_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 141, 64)) break;
         if (lane == 0) mbar_arrive_expect_tx(&q_full[s], stage);
         __syncwarp();
         uint8_t* dst = s_qg + s * stage + lane * kExQChunk;
@@ -800,7 +826,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       // ------------------------------------------------- statistics of the steps' queries
       for (int i = 0; i < n; i++) {
         const int s = i % kExQStages;
-        if (!mbar_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 149, 64)) break;
+        mbar_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 149, 64);
         float v[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int z = 0; z < 2; z++) {
@@ -822,11 +848,10 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
     const int cw = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const int row = k0 + (warp % 4) * 32 + lane;
-    bool ok = true;
     for (int i = 0; i < n; i++) {
       const int s = i % kExQStages, qa = first + i * kExQ;
-      if (!(ok = mbar_wait(&st_full[s], (i / kExQStages) & 1, abort_flag, a.st, 150))) break;
-      if (!(ok = mbar_wait(sp_full, i & 1, abort_flag, a.st, 151))) break;
+      mbar_wait(&st_full[s], (i / kExQStages) & 1, abort_flag, a.st, 150);
+      mbar_wait(sp_full, i & 1, abort_flag, a.st, 151);
       tc_fence_after();
       uint32_t x[32], y[32];
       ld32(tmem + lanes + cw * 32, x);
@@ -847,7 +872,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           const float4 sd = stat[c / 2];
-          const PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y), make_float2(sd.z, sd.w));
+          const PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y),
+                                    make_float2(sd.z, sd.w));
           pw[c / 2] = Num<T>::pack(r.p.x, r.p.y);
           dw[c / 2] = Num<T>::pack(r.ds.x, r.ds.y);
         }
@@ -856,13 +882,14 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           const float4 sd = stat[c / 2];
-          const PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y), make_float2(sd.z, sd.w));
+          const PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y),
+                                    make_float2(sd.z, sd.w));
           const bool u = c >= from && c < to, v = c + 1 >= from && c + 1 < to;
           pw[c / 2] = Num<T>::pack(u ? r.p.x : 0.f, v ? r.p.y : 0.f);
           dw[c / 2] = Num<T>::pack(u ? r.ds.x : 0.f, v ? r.ds.y : 0.f);
         }
       }
-      if (i > 0 && !(ok = mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 152))) break;
+      if (i > 0) mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 152);
       tc_fence_after();
       tmem_st16(tmem + 448 + lanes + cw * 16, pw);
       tmem_st16(tmem + 480 + lanes + cw * 16, dw);
@@ -871,7 +898,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_ready);
     }
-    if (ok && n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 153);
+    if (n > 0) mbar_wait(acc_done, (n - 1) & 1, abort_flag, a.st, 153);
     tc_fence_after();
     // every product is done: the key tile (first group) and the value tile (second) are free as stages
     const int w_row = row - lane;
@@ -954,13 +981,19 @@ static int packed_maps(ExTma* tm, const ll_latent_packed* p, uint32_t q_rows = 1
   return LL_OK;
 }
 
+static ExOrder ex_order(int rows, int per_tile, const ll_latent_packed* p) {
+  const int tiles = rows / per_tile + p->B;      // at least the sum of ceil(length / per_tile)
+  const int sms = std::max(1, device_info().sms);
+  return {tiles, p->H, std::min(p->H, std::max(1, (4 * sms + tiles - 1) / tiles))};
+}
+
 static int check_packed(const ll_latent_packed* p) {
   if (!p || p->B < 0 || p->Tq < 0 || p->Tk < 0 || p->H <= 0 || (p->d_n != 64 && p->d_n != 128) ||
       (p->d_v != 64 && p->d_v != 128) || (p->d_r != 0 && p->d_r != 64) || (p->dtype != 1 && p->dtype != 2) ||
       !(p->scale > 0.f))
     return LL_ERR_ARG;
   if (p->B == 0 || (p->Tq == 0 && p->Tk == 0)) return LL_OK;
-  if (!p->cu_q || !p->cu_k || (int64_t)(p->Tq / 128 + p->B) * p->H > INT32_MAX || (int64_t)(p->Tk / 128 + p->B) * p->H > INT32_MAX)
+  if (!p->cu_q || !p->cu_k || ((int64_t)std::max(p->Tq, p->Tk) / 128 + p->B) * p->H > INT32_MAX)
     return LL_ERR_ARG;
   if (p->Tq && bad16(p->q, p->q_stride_t, p->q_stride_h)) return LL_ERR_ARG;
   if (p->Tk && (bad16(p->k_nope, p->k_stride_t, p->k_stride_h) || bad16(p->v, p->v_stride_t, p->v_stride_h) ||
@@ -970,18 +1003,21 @@ static int check_packed(const ll_latent_packed* p) {
 }
 
 template <class T>
-static int run_backward(const ll_latent_packed* p, const ExTma& tq, const ExTma& tk, const ExBwdArgs& a, void* dk_pe,
+static int run_backward(const ll_latent_packed* p, const ExTma& tq, const ExTma& tk, ExBwdArgs& a, void* dk_pe,
                         cudaStream_t s) {
   const int nqk = a.nn + a.nr;
   if (p->Tq) {
     const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 13 * 8 + 16 + 512;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dq<T>), smem));
-    LL_TRY(launch_pdl("k_ex_dq", k_ex_dq<T>, dim3(p->Tq / 128 + p->B, p->H), dim3(kExThreads), smem, s, tq, a));
+    a.order = ex_order(p->Tq, 128, p);
+    LL_TRY(launch_pdl("k_ex_dq", k_ex_dq<T>, dim3(a.order.tiles * p->H), dim3(kExThreads), smem, s, tq, a));
   }
   if (p->Tk) {
-    const int smem = 1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 7) * 8 + 16;
+    const int smem =
+        1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 7) * 8 + 16;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dkv<T>), smem));
-    LL_TRY(launch_pdl("k_ex_dkv", k_ex_dkv<T>, dim3(p->Tk / 128 + p->B, p->H), dim3(kExThreads), smem, s, tk, a));
+    a.order = ex_order(p->Tk, 128, p);
+    LL_TRY(launch_pdl("k_ex_dkv", k_ex_dkv<T>, dim3(a.order.tiles * p->H), dim3(kExThreads), smem, s, tk, a));
     const int64_t n = (int64_t)p->Tk * p->d_r;
     if (n)
       LL_TRY(launch_pdl("k_ex_sum_heads", k_ex_sum_heads<T>, dim3((unsigned)((n + 1023) / 1024)), dim3(256), 0, s,
@@ -1010,12 +1046,12 @@ int ll_latent_forward(const ll_latent_packed* p, void* out, float* lse, void* st
   ExTma tm;
   LL_TRY(packed_maps(&tm, p));
   ExFwdArgs a{p->cu_q, p->cu_k, out, lse, p->B, p->Tq, p->Tk, p->H, p->d_n / 64, p->d_r / 64, p->d_v / 64, p->causal,
-              p->scale * 1.4426950408889634f, latent_status()};
+              ex_order(p->Tq, 256, p), p->scale * 1.4426950408889634f, latent_status()};
   if (!a.st) return LL_ERR_CUDA;
   const int smem = 1024 + (2 * (a.nn + a.nr) + kExRing) * kExChunk + (2 * kExOps + 9) * 8 + 16;
   auto run = [&](auto kern) {
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(kern), smem));
-    return launch_pdl("k_ex_fwd", kern, dim3(p->Tq / 256 + p->B, p->H), dim3(kExThreads), smem, s, tm, a);
+    return launch_pdl("k_ex_fwd", kern, dim3(a.order.tiles * p->H), dim3(kExThreads), smem, s, tm, a);
   };
   return p->dtype == 1 ? run(k_ex_fwd<__nv_bfloat16>) : run(k_ex_fwd<__half>);
 }

@@ -49,6 +49,16 @@ LL_DEV bool elect_one() {
   return r != 0;
 }
 
+// A bounded wait of a whole warp with one outcome: lanes that left a loop apart after a timeout would meet
+// the others' warp-wide instructions no more.
+LL_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, DevStatus* st, int where) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, st, where));
+}
+LL_DEV bool warp_wait_sleep(uint64_t* bar, uint32_t parity, volatile int* abort_flag, DevStatus* st, int where,
+                            uint32_t ns_max) {
+  return __all_sync(0xffffffffu, mbar_wait_sleep(bar, parity, abort_flag, st, where, ns_max));
+}
+
 // More bytes for the current phase to wait for, without arriving.
 LL_DEV void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");

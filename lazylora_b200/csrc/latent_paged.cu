@@ -251,12 +251,12 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         }
         const int off = key % a.page_size;
         // the second product releases a stage by halves, so the first four groups go ahead
-        if (!(ok = mbar_wait(&kv_empty[st * 2], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 81))) break;
+        if (!(ok = warp_wait(&kv_empty[st * 2], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 81))) break;
         if (lane == 0) mbar_expect_tx(&kv_full[st], min(groups, 4) * group_bytes);
         __syncwarp();
         uint8_t* dst = s_kv + st * tile_bytes + lane * group_bytes;
         if (lane < min(groups, 4)) tma_load_4d(dst, &tm.kv, &kv_full[st], 0, off, 0, page);
-        ok = mbar_wait(&kv_empty[st * 2 + 1], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 82);
+        ok = warp_wait(&kv_empty[st * 2 + 1], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 82);
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], ok ? max(groups - 4, 0) * group_bytes : 0);
         __syncwarp();
         if (!ok) { n++; break; }
@@ -297,8 +297,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
 #pragma unroll 1
       for (int j = j0; j < j1; j++, n++) {
         const bool first = j == j0;
-        if (!(ok = mbar_wait(&kv_full[n & 1], (n >> 1) & 1, abort_flag, a.st, 86))) break;
-        if (first && !(ok = mbar_wait(q_full, piece & 1, abort_flag, a.st, 87))) break;
+        if (!(ok = warp_wait(&kv_full[n & 1], (n >> 1) & 1, abort_flag, a.st, 86))) break;
+        if (first && !(ok = warp_wait(q_full, piece & 1, abort_flag, a.st, 87))) break;
         tc_fence_after();
         const uint32_t at = tmem_s + (n & 1) * 64, k0 = k_d.lo + (n & 1) * tile16, v0 = v_d.lo + (n & 1) * tile16;
         if (lead) {
@@ -309,8 +309,8 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
           mma_commit(&s_full[n & 1]);
           if (j == j1 - 1) mma_commit(q_empty);
         }
-        if (!(ok = mbar_wait(p_ready, n & 1, abort_flag, a.st, 88))) break;
-        if (first && piece > 0 && !(ok = mbar_wait(o_free, (piece - 1) & 1, abort_flag, a.st, 89))) break;
+        if (!(ok = warp_wait(p_ready, n & 1, abort_flag, a.st, 88))) break;
+        if (first && piece > 0 && !(ok = warp_wait(o_free, (piece - 1) & 1, abort_flag, a.st, 89))) break;
         tc_fence_after();
         if (lead) {
 #pragma unroll
