@@ -25,9 +25,9 @@ namespace ll {
 // cores' operand, the output's own precision); sums in fp32 of the unrounded values.
 constexpr int kExThreads = 384;        // warps 0-3, 4-7: softmax of tile 0, 1; 8: TMA; 9: MMA; 10, 11: none
 // Registers: launched with 168 a thread (64,512 a block); the third warpgroup gives some of its up to the two
-// softmax warpgroups: 216 * 256 + 72 * 128 = 176 * 256 + 152 * 128 = 64,512. (The backward's loading and issuing
+// softmax warpgroups: 224 * 256 + 56 * 128 = 176 * 256 + 152 * 128 = 64,512. (The backward's loading and issuing
 // warps spill below 152, 4 % of a packed step; its element-wise warps need no more than 176.)
-constexpr int kExRegsMore = 216, kExRegsLess = 72, kExBwdMore = 176, kExBwdLess = 152;
+constexpr int kExRegsMore = 224, kExRegsLess = 56, kExBwdMore = 176, kExBwdLess = 152;
 constexpr int kExRing = 8;
 constexpr int kExChunk = 128 * 128;    // bytes
 constexpr int kExOps = 16;             // barriers of the ring's operands
