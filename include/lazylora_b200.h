@@ -395,7 +395,7 @@ int ll_latent_rotate(const void* x, int64_t x_stride_t, int64_t x_stride_h, cons
  *   s_j = scale * q . row_j,  p = softmax(s),  out [B][Tq][H][d_c] = sum_j p_j row_j[0 .. d_c),
  *   lse [B][Tq][H] = log sum_j exp(s_j); a query that sees nothing gets zeros and -inf.
  * Query row t * H + h of sequence b starts at b * q_stride_b + (t * H + h) * q_stride_row. d_c 128,
- * 256, 384 or 512; d_r 0 or 64; page_size a multiple of 8. out and lse contiguous.
+ * 256, 384 or 512; d_r 0 or 64; page_size a multiple of 8; scale > 0. out and lse contiguous.
  * Workspace of ll_paged_latent_workspace_bytes, needed until the call's kernels have run. */
 size_t ll_paged_latent_workspace_bytes(int B, int Tq, int H, int d_c);
 int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_stride_row, const void* cache,
@@ -407,8 +407,8 @@ int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_strid
 /* The expanded form on packed sequences: queries q [Tq][H][d_n + d_r], keys k_nope [Tk][H][d_n]
  * beside the shared k_pe [Tk][d_r], values v [Tk][H][d_v]; sequence b holds query rows cu_q[b] ..
  * cu_q[b + 1] and key rows cu_k[b] .. cu_k[b + 1] (int32 [B + 1], device). With causal, query i of
- * a sequence sees its keys j <= i + (keys - queries), else all of them. d_n and d_v 64 or 128, d_r
- * 0 or 64. */
+ * a sequence sees its keys j <= i + (keys - queries), else all of them. The sequences cover all rows (rows
+ * outside every sequence are neither read nor written). d_n and d_v 64 or 128, d_r 0 or 64; scale > 0. */
 typedef struct {
   int B, Tq, Tk, H, d_n, d_r, d_v;
   int causal, dtype;

@@ -11,6 +11,8 @@
 // pieces), or 8 latent values to copy. A thread requests its first four items before the token's position
 // and its table row (which the heads share through L1) have arrived: three dependent loads become two.
 // Offsets are 64-bit: a cache passes 2^32 bytes.
+// Measured: 9001 tokens with 64 heads (171 MB) 38 us, 4.5 TB/s, 69 % of the copy rate (four items ahead: 56 us, 320
+// threads: 46 us); a decode step of 40 tokens 2.9 us.
 #include "latent_ops.cuh"
 
 namespace ll {

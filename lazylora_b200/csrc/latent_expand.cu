@@ -10,7 +10,9 @@ namespace ll {
 
 // ------------------------------------------------------------------------------- forward
 // One CTA takes 256 query rows of one sequence and head as two tiles of 128 that alternate: while one
-// tile's softmax runs, the tensor cores do the other's products.
+// tile's softmax runs, the tensor cores do the other's products. Measured: 8000 tokens at 32 heads (655
+// GFLOP) 565 us, 1.16 PFLOP/s; in a loop that holds the power limit (1000 W, 1.7 GHz) 647 us, 70 % of
+// what a large cuBLAS product sustains there.
 //   S_t [128][128 keys] = Q_t K^T       (M = 128, N = 128, K = d_n + d_r)
 //   O_t [128][d_v]     += P_t V         (P_t from tensor memory)
 // Issue order per key tile i: O_0(i - 1), S_0(i), O_1(i - 1), S_1(i). Per 256 x 128 scores at 192 / 128 that
@@ -388,8 +390,11 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
 // cores one step ahead of the element-wise work, which turns S and dP into P and dS:
 //   issue order  S(i + 1), dP(i + 1), then the sums over step i.
 // P and dS reach the tensor cores through tensor memory, rounded to the 16-bit type (as the gradients
-// themselves); scale is applied to the fp32 sums. Per step the products take 2048 (dq: 128 keys) and
-// about 1400 cycles (dk, dv: 64 queries) against 1024 and 512 of exponentials.
+// themselves); scale is applied to the fp32 sums.
+// Per step the products take 2048 (dq: 128 keys) and about 1400 cycles (dk, dv: 64 queries) against 1024 and
+// 512 of exponentials; measured 3000 and 1900. 4100 tokens at 64 heads: 0.59 ms (dq) and 0.68 ms (dk, dv); 7
+// documents of 150 to 1024 tokens: 0.20 and 0.23 ms, half of it the blocks' first loads (120 KB, 5000 cycles
+// with the set-up) and stores (3000).
 //
 // Tensor memory, 512 columns each:
 //   dq:     S 0 (128), dP 128 (128), dQ 256 (192), dS 448 (64)
