@@ -469,7 +469,10 @@ def run_ours(args, cfg, rank, local, world, dist):
         line["single_gpu_same_workload_ms"] = single_ms
         line["strong_efficiency"] = single_ms / (world * ms_step) if single_ms else None
         line["all_to_all"] = a2a
-    if args.cpu_baseline and world == 1:
+    from oracle import moe_oracle as O
+    if args.cpu_baseline and world == 1 and not os.path.exists(O.REF_SO):
+        line["cpu_baseline"] = {"unavailable": "the reference's C kernel (oracle/_ref) has not been compiled here"}
+    elif args.cpu_baseline and world == 1:
         weights = {"w1p": layer.w1p, "w3p": layer.w3p, "w2p": layer.w2p, "w1s": layer.w1s[..., :cfg.d // 32],
                    "w3s": layer.w3s[..., :cfg.d // 32], "w2s": layer.w2s[..., :cfg.f // 32]}
         dt, frac, threads = cpu_reference_sample(cfg, {**inp, **weights}, idx, res[5], None)
