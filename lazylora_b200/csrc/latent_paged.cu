@@ -46,7 +46,6 @@ namespace ll {
 constexpr int kPgSoft = 256;           // softmax threads: warps 0-7; warp 8: TMA, warp 9: MMA
 constexpr int kPgThreads = kPgSoft + 64;
 constexpr int kPgKeys = 64;
-constexpr int kPgStages = 6;           // at most
 constexpr float kPgSlack = 8.f;        // log2 of how far a score may pass its row's reference
 constexpr float kPgNone = -1e30f;      // reference of a row that has seen no key
 
@@ -59,7 +58,7 @@ struct PagedArgs {
   float* part_ml;     // [G * 2][RT][2][NT] their references (log2) and sums
   int* starts;        // [B + 1] weight before each sequence; last: weight of a range
   int64_t bt_stride;
-  int pages, page_size, max_pages, B, Tq, H, rows, RT, G, stages, nc, nchunk;   // chunks of 64: of d_c, of d_c + d_r
+  int pages, page_size, max_pages, B, Tq, H, rows, RT, G, nc, nchunk;   // chunks of 64: of d_c, of d_c + d_r
   float scale_log2;
   DevStatus* st;
 };
@@ -173,14 +172,13 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int nchunk = a.nchunk, group_bytes = nchunk * 1024, tile_bytes = 8 * group_bytes;
-  uint8_t* s_kv = base;                               // a.stages tiles
-  uint8_t* s_q = s_kv + a.stages * tile_bytes;               // [chunk][NT rows][128 bytes]
+  uint8_t* s_kv = base;                               // two tiles
+  uint8_t* s_q = s_kv + 2 * tile_bytes;               // [chunk][NT rows][128 bytes]
   uint8_t* s_p = s_q + nchunk * NT * 128;             // [64 keys][128 bytes]: P^T, rows of NT values
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_p + kPgKeys * 128);
-  uint64_t *kv_full = bars, *kv_empty = kv_full + kPgStages, *s_full = kv_empty + 2 * kPgStages, *q_full = s_full + 2,
-           *q_empty = s_full + 3, *p_ready = s_full + 4, *o_done = s_full + 5, *o_free = s_full + 6, *drain = s_full + 7;
-  constexpr int kBars = 3 * kPgStages + 10;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
+  uint64_t *kv_full = bars, *kv_empty = bars + 2, *s_full = bars + 6, *q_full = bars + 8, *q_empty = bars + 9,
+           *p_ready = bars + 10, *o_done = bars + 11, *o_free = bars + 12, *drain = bars + 13;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 14);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_start = reinterpret_cast<int*>(tmem_slot + 2);        // first sequence, first tile of it, tiles before, after
   float* s_red = reinterpret_cast<float*>(tmem_slot + 8);              // [4 warps][64]
@@ -190,7 +188,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   const int g = blockIdx.x / a.RT, rt = blockIdx.x % a.RT;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBars - 1; i++) mbar_init(&bars[i], &bars[i] == p_ready || &bars[i] == o_free ? kPgSoft / 32 : 1);
+    for (int i = 0; i < 14; i++) mbar_init(&bars[i], i == 10 || i == 12 ? kPgSoft / 32 : 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -247,12 +245,11 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     // Lane i takes the tile's group i of eight keys: it looks its page up while the stage is still in
     // use, then issues its own box.
     bool ok = true;
-    uint32_t n = 0, seg = 0, q_loads = 0, ph = 0;
-    int st = 0;
+    uint32_t n = 0, seg = 0, q_loads = 0;
     for (; w.left > 0 && ok; w.next(a), seg++) {
       const int j0 = w.j, j1 = w.end();
-      for (int j = j0; j < j1; j++) {
-        const int key = j * kPgKeys + lane * 8;
+      for (int j = j0; j < j1; j++, n++) {
+        const int st = n & 1, key = j * kPgKeys + lane * 8;
         const int groups = (min(kPgKeys, max(0, w.len - j * kPgKeys)) + 7) / 8;
         int page = a.pages;                       // outside the map: reads zeros
         if (lane < groups) {
@@ -262,36 +259,31 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         }
         const int off = key % a.page_size;
         // the second product releases a stage by halves, so the first four groups go ahead
-        if (!(ok = warp_wait(&kv_empty[st * 2], ph ^ 1, abort_flag, a.st, 81))) break;
+        if (!(ok = warp_wait(&kv_empty[st * 2], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 81))) break;
         if (lane == 0) mbar_expect_tx(&kv_full[st], min(groups, 4) * group_bytes);
         __syncwarp();
         uint8_t* dst = s_kv + st * tile_bytes + lane * group_bytes;
         if (lane < min(groups, 4)) tma_load_4d(dst, &tm.kv, &kv_full[st], 0, off, 0, page);
-        ok = warp_wait(&kv_empty[st * 2 + 1], ph ^ 1, abort_flag, a.st, 82);
+        ok = warp_wait(&kv_empty[st * 2 + 1], ((n >> 1) & 1) ^ 1, abort_flag, a.st, 82);
         if (lane == 0) mbar_arrive_expect_tx(&kv_full[st], ok ? max(groups - 4, 0) * group_bytes : 0);
         __syncwarp();
-        n++;
-        uint64_t* full = &kv_full[st];
-        if (++st == a.stages) { st = 0; ph ^= 1; }
-        if (!ok) break;
-        if (lane >= 4 && lane < groups) tma_load_4d(dst, &tm.kv, full, 0, off, 0, page);
+        if (!ok) { n++; break; }
+        if (lane >= 4 && lane < groups) tma_load_4d(dst, &tm.kv, &kv_full[st], 0, off, 0, page);
         if (j == j0) {
           if (lane == 0) {
             ok = mbar_wait(q_empty, (seg & 1) ^ 1, abort_flag, a.st, 80);
             if (ok) mbar_arrive_expect_tx(q_full, nchunk * NT * 128);
           }
           ok = __shfl_sync(0xffffffffu, ok, 0);
-          if (!ok) break;
+          if (!ok) { n++; break; }
           q_loads++;
           if (lane < nchunk) tma_load_3d(s_q + lane * NT * 128, &tm.q, q_full, lane * 64, rt * NT, w.b);
         }
       }
     }
     volatile int keep = 0;                        // what was issued has landed, also after an abort
-    for (uint32_t i = 0; i < min(n, (uint32_t)a.stages); i++) {
-      if (--st < 0) { st = a.stages - 1; ph ^= 1; }
-      mbar_wait_sleep(&kv_full[st], ph, &keep, a.st, 83, 64);
-    }
+    if (n >= 1) mbar_wait_sleep(&kv_full[(n - 1) & 1], ((n - 1) >> 1) & 1, &keep, a.st, 83, 64);
+    if (n >= 2) mbar_wait_sleep(&kv_full[n & 1], ((n - 2) >> 1) & 1, &keep, a.st, 84, 64);
     if (q_loads >= 1) mbar_wait_sleep(q_full, (q_loads - 1) & 1, &keep, a.st, 85, 64);
     __syncwarp();
   } else if (warp == 9) {
@@ -306,18 +298,17 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     const MmaDesc k_d(smem_u32(s_kv), 16, group_bytes), v_d(smem_u32(s_kv), 1024, group_bytes);
     const uint32_t tile16 = tile_bytes >> 4, group16 = group_bytes >> 4;
     const int mts = a.nc / 2;
-    uint32_t n = 0, piece = 0, ph = 0;
-    int st = 0;
+    uint32_t n = 0, piece = 0;
     bool ok = true;
     for (; w.left > 0 && ok; w.next(a), piece++) {
       const int j0 = w.j, j1 = w.end();
 #pragma unroll 1
       for (int j = j0; j < j1; j++, n++) {
         const bool first = j == j0;
-        if (!(ok = warp_wait(&kv_full[st], ph, abort_flag, a.st, 86))) break;
+        if (!(ok = warp_wait(&kv_full[n & 1], (n >> 1) & 1, abort_flag, a.st, 86))) break;
         if (first && !(ok = warp_wait(q_full, piece & 1, abort_flag, a.st, 87))) break;
         tc_fence_after();
-        const uint32_t at = tmem_s + (n & 1) * 64, k0 = k_d.lo + st * tile16, v0 = v_d.lo + st * tile16;
+        const uint32_t at = tmem_s + (n & 1) * 64, k0 = k_d.lo + (n & 1) * tile16, v0 = v_d.lo + (n & 1) * tile16;
         if (lead) {
           for (int c = 0; c < nchunk; c++)
 #pragma unroll
@@ -339,11 +330,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
                 if (mt < mts)
                   mma_16bit(tmem + mt * NT, v0 + kk * 2 * group16 + mt * 128, v_d.hi, p_d.lo + kk * 128, p_d.hi, id_o,
                             first && kk == 0 ? 0 : 1);
-            mma_commit(&kv_empty[st * 2 + half]);
+            mma_commit(&kv_empty[(n & 1) * 2 + half]);
           }
           if (j == j1 - 1) mma_commit(o_done);
         }
-        if (++st == a.stages) { st = 0; ph ^= 1; }
       }
     }
     __syncwarp();
@@ -361,7 +351,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     const int t0 = (rt * NT + r0) / a.H, h0 = (rt * NT + r0) % a.H;
     uint8_t* p_row = s_p + (key_in / 8) * 1024 + (key_in % 8) * 128;
     uint32_t n = 0, piece = 0;
-    int st = 0;
     for (; w.left > 0; w.next(a)) {
       const int j0 = w.j, j1 = w.end();
       float ref[NQ], l[NQ];
@@ -452,7 +441,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
           const int from = max(valid, 0), per_row = a.nc * 8;
           for (int i = threadIdx.x; i < (kPgKeys - from) * per_row; i += kPgSoft) {
             const int r = from + i / per_row, c = i % per_row;
-            *reinterpret_cast<uint4*>(s_kv + st * tile_bytes + (r / 8) * group_bytes + (c / 8) * 1024 + (r % 8) * 128 +
+            *reinterpret_cast<uint4*>(s_kv + (n & 1) * tile_bytes + (r / 8) * group_bytes + (c / 8) * 1024 + (r % 8) * 128 +
                                       (c % 8) * 16) = make_uint4(0, 0, 0, 0);
           }
         }
@@ -460,7 +449,6 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready);
-        if (++st == a.stages) st = 0;
       }
       // the piece's sums over its keys, in a fixed order
       const int c0 = r0 + fold16<NQ, 8>(l, lane, [](float p, float q) { return p + q; });
@@ -624,11 +612,8 @@ static int launch_paged(const PagedTma& tm, const PagedArgs& a, int smem, cudaSt
 }
 
 template <class T>
-static int run_paged(const PagedTma& tm, PagedArgs& a, int NT, cudaStream_t s) {
-  // as many tiles in flight as fit beside the queries (two at 512 + 64 values and 48 or 64 rows)
-  const int fixed = 1024 + a.nchunk * NT * 128 + kPgKeys * 128 + (3 * kPgStages + 10) * 8 + 32 + 4 * 384;
-  a.stages = std::min(kPgStages, (227 * 1024 - fixed) / (a.nchunk * 8192));
-  const int smem = fixed + a.stages * a.nchunk * 8192;
+static int run_paged(const PagedTma& tm, const PagedArgs& a, int NT, cudaStream_t s) {
+  const int smem = 1024 + 2 * a.nchunk * 8192 + a.nchunk * NT * 128 + kPgKeys * 128 + 144 + 4 * 384;
   if (NT == 16) LL_TRY((launch_paged<T, 16>(tm, a, smem, s)));
   else if (NT == 32) LL_TRY((launch_paged<T, 32>(tm, a, smem, s)));
   else if (NT == 48) LL_TRY((launch_paged<T, 48>(tm, a, smem, s)));
