@@ -391,6 +391,12 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
 //   issue order  S(i + 1), dP(i + 1), then the sums over step i.
 // P and dS reach the tensor cores through tensor memory, rounded to the 16-bit type (as the gradients
 // themselves); scale is applied to the fp32 sums.
+// fp16 holds dS = P (dP - delta) up to 65504 only, where the gradients, after the scale and the sums, may be far
+// within the type. So in fp16 a row of dS is held times a power of two, 1 until one of its values passes the
+// type; then the row's largest value comes to 2^14 .. 2^15, and the sums so far with it. Ordinary values are as
+// without it; a step's check costs fp16 4 to 7 % (forward and backward of 4100 tokens at 64 heads 1645 -> 1707 us,
+// of 7 documents 635 -> 680; a vote of all 256 threads and the largest value itself 1818 and 690). bf16 has
+// fp32's range.
 // Per step the products take 2048 (dq: 128 keys) and about 1400 cycles (dk, dv: 64 queries) against 1024 and
 // 512 of exponentials; measured 3000 and 1900. 4100 tokens at 64 heads: 0.59 ms (dq) and 0.68 ms (dk, dv); 7
 // documents of 150 to 1024 tokens: 0.20 and 0.23 ms, half of it the blocks' first loads (120 KB, 5000 cycles
@@ -435,6 +441,50 @@ LL_DEV void zero_tail(uint8_t* at, int chunks, int rows, int from) {
   }
 }
 
+// A row's factor for a step whose dS this thread holds N values of (d, their squares' sum sq): f, or less when a
+// value passes fp16's range. Threads t and t + 128 share row t of the tile, so their two warps vote; the sum of
+// squares, one packed operation for two values, stands for the largest value until it passes the limit. The
+// row's sums so far, `cols` columns from `acc` on, are brought to the new factor once `summed` has waited for them
+// (false: there are none). A row that holds an infinity keeps its factor: its gradient is not finite either.
+template <int N, class Summed>
+LL_DEV float ds_factor(const uint32_t* d, float sq, float f, float* s_top, uint32_t acc, int cols, Summed summed) {
+  constexpr float kMost = 65504.f;
+  const int t = threadIdx.x, pair = 2 + t / 32 % 4;
+  if (!bar_any<64>(pair, !(sq * (f * f) <= kMost * kMost))) return f;
+  float m = 0.f;
+#pragma unroll
+  for (int c = 0; c < N; c++) m = fmaxf(m, fabsf(__uint_as_float(d[c])));
+  s_top[t] = m * f;
+  named_bar_sync(pair, 64);
+  const float top = fmaxf(s_top[t % 128], s_top[t % 128 + 128]);
+  // 2^(14 - e) for top = 2^e .. 2^(e + 1)
+  const float less = top > kMost && top < INFINITY ? __uint_as_float((268u - (__float_as_uint(top) >> 23)) << 23) : 1.f;
+  if (summed()) {
+    for (int c = t / 128 * 32; c < cols; c += 64) {
+      uint32_t o[32];
+      ld32(acc + c, o);
+      tmem_ld_wait();
+      ld32_ready(o);
+#pragma unroll
+      for (int k = 0; k < 32; k++) o[k] = __float_as_uint(__uint_as_float(o[k]) * less);
+      st32(acc + c, o);
+    }
+    tmem_st_wait();
+  }
+  return f * less;
+}
+// N values of dS, times their row's factor, as words of the 16-bit type.
+template <class T, int N>
+LL_DEV void pack_ds(const uint32_t* d, float f, uint32_t* w) {
+  if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) w[c / 2] = Num<T>::pack(__uint_as_float(d[c]) * f, __uint_as_float(d[c + 1]) * f);
+  } else {
+#pragma unroll
+    for (int c = 0; c < N; c += 2) w[c / 2] = Num<T>::pack(__uint_as_float(d[c]), __uint_as_float(d[c + 1]));
+  }
+}
+
 template <class T>
 __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__ ExTma tm, const ExBwdArgs a) {
   extern __shared__ uint8_t smem_raw[];
@@ -449,7 +499,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
            *sp_full = bars + 7, *sp_free = bars + 8, *ds_ready = bars + 9, *acc_done = bars + 10, *drain = bars + 11;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 13);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  float* s_delta = reinterpret_cast<float*>(tmem_slot + 4);
+  float* s_delta = reinterpret_cast<float*>(tmem_slot + 4);      // [128], read before the steps; in them [256] of ds_factor
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   int tile, head;
   ex_deal(a.order, tile, head);
@@ -619,6 +669,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       lse2 = a.lse[at] * 1.4426950408889634f;
       if (cw == 0) a.delta[at] = delta;
     }
+    float f = 1.f;                             // dS's factor (fp16)
     for (int i = 0; i < n; i++) {
       mbar_wait(sp_full, i & 1, abort_flag, a.st, 132);
       tc_fence_after();
@@ -642,7 +693,28 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
         fence_async_smem();
       }
       uint32_t w[32];
-      if (i * 128 + 128 <= see_all) {          // every row sees every key
+      if constexpr (Num<T>::narrow) {
+        float2 sq = make_float2(0.f, 0.f);
+        auto compute = [&](int lim) {
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) {
+            float2 d = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(-lse2, -lse2),
+                                make_float2(-delta, -delta)).ds;
+            d = make_float2(c < lim ? d.x : 0.f, c + 1 < lim ? d.y : 0.f);
+            sq = fma2(d, d, sq);
+            x[c] = __float_as_uint(d.x);
+            x[c + 1] = __float_as_uint(d.y);
+          }
+        };
+        if (i * 128 + 128 <= see_all) compute(64);       // every row sees every key
+        else compute(see - i * 128 - cw * 64);
+        f = ds_factor<64>(x, row < nq ? sq.x + sq.y : 0.f, f, s_delta, tmem + 256 + lanes, nqk * 64, [&] {
+          if (i > 0) mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 136);
+          tc_fence_after();
+          return i > 0;
+        });
+        pack_ds<T, 64>(x, f, w);
+      } else if (i * 128 + 128 <= see_all) {   // every row sees every key
 #pragma unroll
         for (int c = 0; c < 64; c += 2) {
           const float2 d = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(-lse2, -lse2),
@@ -674,7 +746,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
     uint8_t* dst = static_cast<uint8_t*>(a.dq) + ((int64_t)(q_lo + w_row) * a.H + head) * (nqk * 128);
     for (int c = cw; c < nqk; c += 2) {
       uint32_t w[32];
-      load_acc64<T>(tmem + 256 + lanes + c * 64, n > 0, a.scale, w);
+      load_acc64<T>(tmem + 256 + lanes + c * 64, n > 0, a.scale / f, w);
       store_rows(stage, w, lane, nq - w_row, dst + c * 128, (int64_t)a.H * (nqk * 128));
     }
   }
@@ -703,6 +775,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
            *drain = sp_full + 4;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* s_top = reinterpret_cast<float*>(tmem_slot + 4);        // [256] of ds_factor
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   int tile, head;
   ex_deal(a.order, tile, head);
@@ -853,6 +926,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
     const int cw = warp / 4;
     const uint32_t lanes = (uint32_t)((warp % 4) * 32) << 16;
     const int row = k0 + (warp % 4) * 32 + lane;
+    float f = 1.f;                             // dS's factor (fp16)
     for (int i = 0; i < n; i++) {
       const int s = i % kExQStages, qa = first + i * kExQ;
       mbar_wait(&st_full[s], (i / kExQStages) & 1, abort_flag, a.st, 150);
@@ -873,7 +947,31 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       }
       uint32_t pw[16], dw[16];
       const float4* stat = s_stat + s * 32 + cw * 16;
-      if (qa + kExQ <= nq && (!a.causal || k0 + 127 <= qa + shift)) {     // every query sees every row
+      if constexpr (Num<T>::narrow) {
+        float2 sq = make_float2(0.f, 0.f);
+        auto compute = [&](int from, int to) {           // the queries that see the row
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const float4 sd = stat[c / 2];
+            PAndDs r = p_and_ds(x[c], x[c + 1], y[c], y[c + 1], a.scale_log2, make_float2(sd.x, sd.y),
+                                make_float2(sd.z, sd.w));
+            const bool u = c >= from && c < to, v = c + 1 >= from && c + 1 < to;
+            r.ds = make_float2(u ? r.ds.x : 0.f, v ? r.ds.y : 0.f);
+            sq = fma2(r.ds, r.ds, sq);
+            pw[c / 2] = Num<T>::pack(u ? r.p.x : 0.f, v ? r.p.y : 0.f);
+            y[c] = __float_as_uint(r.ds.x);
+            y[c + 1] = __float_as_uint(r.ds.y);
+          }
+        };
+        if (qa + kExQ <= nq && (!a.causal || k0 + 127 <= qa + shift)) compute(0, 32);
+        else compute((a.causal ? row - shift - qa : 0) - cw * 32, nq - qa - cw * 32);
+        f = ds_factor<32>(y, row < nk ? sq.x + sq.y : 0.f, f, s_top, tmem + 256 + lanes, nqk * 64, [&] {
+          if (i > 0) mbar_wait(acc_done, (i - 1) & 1, abort_flag, a.st, 155);
+          tc_fence_after();
+          return i > 0;
+        });
+        pack_ds<T, 32>(y, f, dw);
+      } else if (qa + kExQ <= nq && (!a.causal || k0 + 127 <= qa + shift)) {     // every query sees every row
 #pragma unroll
         for (int c = 0; c < 32; c += 2) {
           const float4 sd = stat[c / 2];
@@ -913,7 +1011,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       const bool v = c < a.nv;
       const int cc = v ? c : c - a.nv, chunks = v ? a.nv : a.nn;
       uint32_t w[32];
-      load_acc64<T>(tmem + lanes + (v ? 128 : 256) + cc * 64, n > 0, v ? 1.f : a.scale, w);
+      load_acc64<T>(tmem + lanes + (v ? 128 : 256) + cc * 64, n > 0, v ? 1.f : a.scale / f, w);
       store_rows(stage, w, lane, nk - w_row, static_cast<uint8_t*>(v ? a.dv : a.dk) + at * (chunks * 128) + cc * 128,
                  (int64_t)a.H * (chunks * 128));
     }
@@ -925,7 +1023,7 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
         ld32_ready(w);
       }
 #pragma unroll
-      for (int k = 0; k < 32; k++) w[k] = n > 0 ? __float_as_uint(__uint_as_float(w[k]) * a.scale) : 0u;
+      for (int k = 0; k < 32; k++) w[k] = n > 0 ? __float_as_uint(__uint_as_float(w[k]) * (a.scale / f)) : 0u;
       store_rows(stage, w, lane, nk - w_row,
                  reinterpret_cast<uint8_t*>(a.dkpe + ((int64_t)head * a.Tk + k_lo + w_row) * (a.nr * 64) + c), a.nr * 256);
     }
@@ -1012,14 +1110,14 @@ static int run_backward(const ll_latent_packed* p, const ExTma& tq, const ExTma&
                         cudaStream_t s) {
   const int nqk = a.nn + a.nr;
   if (p->Tq) {
-    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 13 * 8 + 16 + 512;
+    const int smem = 1024 + (3 * nqk + 2 * a.nv) * kExChunk + 13 * 8 + 16 + 1024;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dq<T>), smem));
     a.order = ex_order(p->Tq, 128, p);
     LL_TRY(launch_pdl("k_ex_dq", k_ex_dq<T>, dim3(a.order.tiles * p->H), dim3(kExThreads), smem, s, tq, a));
   }
   if (p->Tk) {
     const int smem =
-        1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 7) * 8 + 16;
+        1024 + (nqk + a.nv) * (kExChunk + kExQStages * kExQChunk) + kExQStages * 512 + (3 * kExQStages + 7) * 8 + 16 + 1024;
     LL_TRY(set_smem_attr(reinterpret_cast<const void*>(k_ex_dkv<T>), smem));
     a.order = ex_order(p->Tk, 128, p);
     LL_TRY(launch_pdl("k_ex_dkv", k_ex_dkv<T>, dim3(a.order.tiles * p->H), dim3(kExThreads), smem, s, tk, a));

@@ -17,6 +17,7 @@ struct Num;
 template <>
 struct Num<__nv_bfloat16> {
   static constexpr uint32_t fmt = 1;     // kind::f16 operand format code
+  static constexpr bool narrow = false;  // a range short of fp32's
   static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   LL_DEV static float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
   LL_DEV static __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
@@ -28,6 +29,7 @@ struct Num<__nv_bfloat16> {
 template <>
 struct Num<__half> {
   static constexpr uint32_t fmt = 0;
+  static constexpr bool narrow = true;
   static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   LL_DEV static float to_f(__half v) { return __half2float(v); }
   LL_DEV static __half from_f(float v) { return __float2half_rn(v); }
@@ -57,6 +59,19 @@ LL_DEV bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, 
 LL_DEV bool warp_wait_sleep(uint64_t* bar, uint32_t parity, volatile int* abort_flag, DevStatus* st, int where,
                             uint32_t ns_max) {
   return __all_sync(0xffffffffu, mbar_wait_sleep(bar, parity, abort_flag, st, where, ns_max));
+}
+
+// Barrier `id` of N threads, with a vote: whether p holds for any of them.
+template <int N>
+LL_DEV bool bar_any(int id, bool p) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
+      "bar.red.or.pred q, %2, %3, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)p), "r"(id), "n"(N)
+      : "memory");
+  return r != 0;
 }
 
 // More bytes for the current phase to wait for, without arriving.

@@ -132,18 +132,6 @@ LL_DEV int fold16(float* v, int lane, Op op) {
   }
 }
 
-// Barrier 1 of the softmax threads, with a vote.
-LL_DEV bool softmax_any(bool p) {
-  uint32_t r;
-  asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\t"
-      "bar.red.or.pred q, 1, 256, p;\n\tselp.b32 %0, 1, 0, q;\n\t}"
-      : "=r"(r)
-      : "r"((uint32_t)p)
-      : "memory");
-  return r != 0;
-}
-
 // The pieces [j, j_end) of sequence b, one after another, that make up a CTA's range of tiles.
 struct PagedWalk {
   int left, b, j, n, len;
@@ -380,7 +368,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
         float top = v[0];
 #pragma unroll
         for (int c = 1; c < NQ; c++) top = fmaxf(top, v[c]);
-        const bool slow = softmax_any(top > kPgSlack);
+        const bool slow = bar_any<kPgSoft>(1, top > kPgSlack);
         if (slow) {
           // new references: each row's maximum so far
           load_scores<NQ>(s_at, v);

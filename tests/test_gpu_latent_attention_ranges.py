@@ -1,0 +1,95 @@
+"""
+The latent-attention operators at the ends of their ranges: lengths and pages that only the device can see
+to be wrong, gradients past fp16's range, empty batches. Each is recorded or computed, never passed over.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_latent_attention import HF, U, _expand_case, _within
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------------------------------- expanded
+def _wide(seed, ql, kl, grow):
+    """fp16 operands whose P (dP - delta) passes 65504 while the gradients, which carry the scale and small
+    queries and keys, do not: |g| about 4000 and |v| about 32, or |g| about 1500, both growing along the rows
+    (later steps raise the largest value again); |q| and |k| about 1/256; every third query's gradient is
+    a thousandth of that."""
+    gen, H = torch.Generator().manual_seed(seed), 2
+    new = lambda n, std, *s: torch.randn(n, *s, generator=gen) * std  # noqa: E731
+    up = lambda n: 1 + torch.arange(n)[:, None, None] / 40 if grow else 1.0  # noqa: E731
+    n, m = sum(ql), sum(kl)
+    small = torch.where(torch.arange(n) % 3 == 1, 1e-3, 1.0)[:, None, None]
+    q, k = new(n, 1 / 256, H, 192), new(m, 1 / 256, H, 128)
+    go = new(n, 1500 if grow else 4000, H, 128) * up(n) * small
+    x = (q, k, new(m, 1 / 256, 64), new(m, 32, H, 128) * up(m), go)
+    q, kn, kp, v, go = (t.to("cuda", HF) for t in x)
+    cum = lambda ls: torch.tensor([sum(ls[:i]) for i in range(len(ls) + 1)], dtype=torch.int32, device="cuda")  # noqa: E731
+    return q, kn, kp, v, cum(ql), cum(kl), go
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("ql,kl,grow", [([40, 3], [40, 3], False), ([300, 70], [300, 70], True), ([65], [400], True)])
+def test_fp16_gradients_whose_unscaled_scores_pass_the_type(ql, kl, grow, causal):
+    """The formula's gradients are finite in fp16 although P (dP - delta), before the scale and the sums,
+    is not. Bound: as derived for ordinary values (dS and P rounded to the type, fp32 scores and sums), where
+    dS is held times a power of two f of its row that brings the row's largest value m to 2^14 .. 2^15
+    when it passes the type: what falls below the type's smallest step is at most 2^-25 / f <= m 2^-39 in
+    dS, twice that beside 2^-24 for the rows that need no factor. The fp32 sums of dP and delta, whose terms
+    cancel where they are large, are off by at most 2^-20 of the sums of their terms' sizes (8 additions of
+    2^-23 each)."""
+    from lazylora_b200.core import latent_attention as A
+    q, kn, kp, v, cq, ck, go = _wide(7, ql, kl, grow)
+    scale, u = 192 ** -0.5, U[HF]
+    out, lse = A.latent_attention_forward(q, kn, kp, v, cq, ck, scale, causal=causal)
+    dq, dkn, dkp, dv = A.latent_attention_backward(go, out, lse, q, kn, kp, v, cq, ck, scale, causal=causal)
+    A.check_status()
+    k = torch.cat([kn, kp[:, None].expand(-1, 2, -1)], -1)
+    Q, K, V, G, O = (t.double().transpose(0, 1) for t in (q, k, v, go, out))
+    want = {n: torch.zeros_like(t) for n, t in (("q", Q), ("k", K), ("v", V))}
+    bound = {n: torch.zeros_like(t) for n, t in want.items()}
+    largest, q0, k0 = 0.0, 0, 0
+    for n, m in zip(ql, kl):
+        a, b = slice(q0, q0 + n), slice(k0, k0 + m)
+        q0, k0 = q0 + n, k0 + m
+        seen = torch.ones(n, m, dtype=torch.bool, device="cuda")
+        seen = seen.tril(m - n) if causal else seen
+        s = (Q[:, a] @ K[:, b].transpose(1, 2) * scale).masked_fill(~seen, -math.inf)
+        p = torch.softmax(s, -1)
+        dp, delta = G[:, a] @ V[:, b].transpose(1, 2), (G[:, a] * O[:, a]).sum(-1, keepdim=True)
+        ds = p * (dp - delta)
+        largest = max(largest, float(ds.abs().max()))
+        terms = G[:, a].abs() @ V[:, b].abs().transpose(1, 2) + (G[:, a] * O[:, a]).abs().sum(-1, keepdim=True)
+        size = p * ((u + 1e-4) * (dp.abs() + delta.abs()) + 2.0 ** -20 * terms)
+        tiny = lambda d: (2.0 ** -24 + ds.abs().amax(d, keepdim=True) * 2.0 ** -38) * seen  # noqa: E731
+        for name, at, x, e, y in (("q", a, ds, size + tiny(2), K[:, b]),
+                                  ("k", b, ds.transpose(1, 2), (size + tiny(1)).transpose(1, 2), Q[:, a])):
+            w = x @ y * scale
+            want[name][:, at] = w
+            bound[name][:, at] = u * w.abs() + scale * (e @ y.abs()) + 2.0 ** -24
+        w = p.transpose(1, 2) @ G[:, a]
+        want["v"][:, b] = w
+        bound["v"][:, b] = u * w.abs() + ((u + 1e-4) * p + 2.0 ** -24 * seen).transpose(1, 2) @ G[:, a].abs() + 2.0 ** -24
+    assert largest > 65504, "the case is about values past the type"
+    w, e = want["k"].transpose(0, 1), bound["k"].transpose(0, 1)
+    kpe = w[..., 128:].sum(1)
+    for got, x, y in ((dq, want["q"].transpose(0, 1), bound["q"].transpose(0, 1)),
+                      (dv, want["v"].transpose(0, 1), bound["v"].transpose(0, 1)), (dkn, w[..., :128], e[..., :128]),
+                      (dkp, kpe, e[..., 128:].sum(1) + u * kpe.abs())):
+        assert float(x.abs().max()) < 65504, "and gradients within it"
+        _within(got, x, y)
+
+
+def test_fp16_gradient_of_one_bad_row_stays_in_it():
+    """An infinite gradient in one query row leaves the other rows' dq as they are without it."""
+    from lazylora_b200.core import latent_attention as A
+    q, kn, kp, v, cq, ck, go = _expand_case(HF, [200], [200], 2, 128, 64, 128, 11)
+    out, lse = A.latent_attention_forward(q, kn, kp, v, cq, ck, 0.07)
+    want = A.latent_attention_backward(go, out, lse, q, kn, kp, v, cq, ck, 0.07)[0]
+    go[37] = float("inf")
+    got = A.latent_attention_backward(go, out, lse, q, kn, kp, v, cq, ck, 0.07)[0]
+    keep = torch.arange(200, device="cuda") != 37
+    assert torch.equal(got[keep], want[keep])
