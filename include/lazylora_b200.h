@@ -367,9 +367,11 @@ const char* ll_profile_launch_name(int i);
  * one rotary key per token (d_r values, shared by the heads). dtype: 1 = bf16, 2 = fp16 for every
  * 16-bit tensor of a call. Strides are in elements, the innermost dimension is contiguous, every
  * pointer is 16-byte aligned and every stride a multiple of 8. Bad device-side values (a position
- * outside the table, a slot outside the cache, a page outside it) are skipped and recorded; a
- * bounded wait that runs out likewise: ll_latent_status(stream) synchronises, returns the first
- * one recorded since the last call on the current device and clears it. */
+ * outside the table, a slot outside the cache, a page outside it, a length that its block table does
+ * not hold) are never followed but recorded; a bounded wait that runs out likewise:
+ * ll_latent_status(stream) synchronises, returns the first one recorded since the last call on the
+ * current device and clears it. A token with a bad position or slot is not written; the attention of a
+ * sequence with a bad value is void. */
 int ll_latent_status(void* stream);
 
 /* New tokens into the paged cache [pages][page_size][d_c + d_r]: token t's row kv[t] (d_c latent

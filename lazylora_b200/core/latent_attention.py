@@ -14,7 +14,7 @@ latent vector per token (d_c values) and one rotary key per token (d_r values, s
 
 bf16 or fp16 tensors, fp32 softmax statistics and sums; CUDA tensors only, no fallback. Calls run on
 the current stream and synchronise nothing; check_status() raises for what only the device can see (a
-position, slot or page out of range). Tensors may be strided: the last dimension contiguous, strides
+position, slot, page or length out of range). Tensors may be strided: the last dimension contiguous, strides
 multiples of 8 elements and 16-byte aligned starts; others are copied once.
 """
 import ctypes
@@ -186,8 +186,9 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
 
     q [B, Tq, H, d_c + d_r]; cache [pages, page_size, d_c + d_r] (page_size a multiple of 8);
     block_table int32 [B, max_pages]; seq_lens int32 [B], the cached rows of each sequence with the
-    Tq queries' own tokens last. Query t of sequence b sees its first seq_lens[b] - Tq + t + 1 rows;
-    one that sees none gets zeros and lse = -inf. d_c 128, 256, 384 or 512; d_r 0 or 64; scale > 0."""
+    Tq queries' own tokens last (0 to max_pages * page_size; others are recorded for check_status()).
+    Query t of sequence b sees its first seq_lens[b] - Tq + t + 1 rows; one that sees none gets zeros and
+    lse = -inf. d_c 128, 256, 384 or 512; d_r 0 or 64; scale > 0."""
     stream = _stream(q, cache, block_table, seq_lens)
     dt = _code(q, cache)
     if q.dim() != 4 or cache.dim() != 3 or q.shape[3] != cache.shape[2]:
@@ -318,6 +319,6 @@ def latent_attention_backward(g: torch.Tensor, out: torch.Tensor, lse: torch.Ten
 
 
 def check_status():
-    """Synchronise and raise if a call since the last check met a position, slot or page out of range
-    (it was skipped) or a bounded wait that ran out."""
+    """Synchronise and raise if a call since the last check met a position, slot, page or length out of range
+    (nothing is read or written outside; a sequence's attention is then void) or a bounded wait that ran out."""
     L.check(L.load().ll_latent_status(L.stream_ptr()), "latent attention")

@@ -67,9 +67,10 @@ struct PagedTma {
   CUtensorMap q, kv;
 };
 
-LL_DEV int paged_len(const PagedArgs& a, int b) {
-  return min(max(a.lens[b], 0), a.max_pages * a.page_size);      // (the host checks that this is an int)
-}
+// (the host checks that this is an int)
+LL_DEV int paged_room(const PagedArgs& a) { return a.max_pages * a.page_size; }
+// A sequence's keys. A length outside the block table, which block 0 records, is cut to it: nothing is read outside.
+LL_DEV int paged_len(const PagedArgs& a, int b) { return min(max(a.lens[b], 0), paged_room(a)); }
 // A sequence without keys still has one (masked) tile, which writes its zeros.
 LL_DEV int paged_tiles(int len) { return max(1, (len - 1) / kPgKeys + 1); }
 // What a sequence weighs in the deal: its tiles, and before them the time that starting and ending it
@@ -209,7 +210,10 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
     if (blockIdx.x == 0 || (first < sum && last >= at))
       for (int b = b_lo; b < b_hi; b++) {
         const int n = paged_tiles(paged_len(a, b)), before = at - kPgStart * b, end = at + n + kPgStart;
-        if (blockIdx.x == 0) a.starts[b] = at;
+        if (blockIdx.x == 0) {
+          a.starts[b] = at;
+          if (a.lens[b] < 0 || a.lens[b] > paged_room(a)) report(a.st, LL_ERR_RANGE, 74, b);
+        }
         if (first >= at && first < end) {
           s_start[0] = b;
           s_start[1] = max(0, first - at - kPgStart);

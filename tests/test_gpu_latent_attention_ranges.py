@@ -7,9 +7,43 @@ import math
 import pytest
 import torch
 
-from test_gpu_latent_attention import HF, U, _expand_case, _within
+from test_gpu_latent_attention import BF, HF, U, _check_paged, _expand_case, _paged_case, _within
 
 pytestmark = pytest.mark.gpu
+
+
+def _raises_once():
+    from lazylora_b200 import _lib as L
+    from lazylora_b200.core import latent_attention as A
+    with pytest.raises(L.LLError, match="out of range"):
+        A.check_status()
+    A.check_status()
+
+
+# ---------------------------------------------------------------------------------------------- paged
+@pytest.mark.parametrize("at,n", [(0, 33), (1, 1000), (2, -1), (0, 2 ** 31 - 1), (1, -2 ** 31)])
+def test_paged_reports_lengths_outside_the_block_table(at, n):
+    """Four pages of eight rows hold 32 keys; one length is past them or negative. The other sequences'
+    outputs are those of the call without it."""
+    from lazylora_b200.core import latent_attention as A
+    q, cache, bt, sl, rows = _paged_case(BF, [20, 24, 9], 1, 4, 128, 64, 8, 2, garbage=0.0)
+    bt = bt.clamp(0, cache.shape[0] - 1)
+    assert bt.shape[1] == 4
+    out, lse = A.paged_latent_attention(q, cache, bt, sl, 128, 0.1)
+    A.check_status()
+    sl[at] = n
+    got, got_lse = A.paged_latent_attention(q, cache, bt, sl, 128, 0.1)
+    _raises_once()
+    others = [b for b in range(3) if b != at]
+    assert torch.equal(got[others], out[others]) and torch.equal(got_lse[others], lse[others])
+
+
+def test_paged_lengths_that_fill_the_block_table_are_fine():
+    from lazylora_b200.core import latent_attention as A
+    q, cache, bt, sl, rows = _paged_case(BF, [32, 0, 31], 2, 4, 128, 64, 8, 3)
+    out, lse = A.paged_latent_attention(q, cache, bt[:, :4].contiguous(), sl, 128, 0.1)
+    A.check_status()
+    _check_paged(out, lse, q, rows, 128, 0.1)
 
 
 # ------------------------------------------------------------------------------------------- expanded
