@@ -409,8 +409,9 @@ int ll_paged_latent_attention(const void* q, int64_t q_stride_b, int64_t q_strid
 /* The expanded form on packed sequences: queries q [Tq][H][d_n + d_r], keys k_nope [Tk][H][d_n]
  * beside the shared k_pe [Tk][d_r], values v [Tk][H][d_v]; sequence b holds query rows cu_q[b] ..
  * cu_q[b + 1] and key rows cu_k[b] .. cu_k[b + 1] (int32 [B + 1], device). With causal, query i of
- * a sequence sees its keys j <= i + (keys - queries), else all of them. The sequences cover all rows (rows
- * outside every sequence are neither read nor written). d_n and d_v 64 or 128, d_r 0 or 64; scale > 0. */
+ * a sequence sees its keys j <= i + (keys - queries), else all of them. The sequences cover all rows:
+ * cu[0] = 0, rising, cu[B] the rows; anything else is recorded (rows outside every sequence are neither
+ * read nor written, as with B = 0). d_n and d_v 64 or 128, d_r 0 or 64; scale > 0. */
 typedef struct {
   int B, Tq, Tk, H, d_n, d_r, d_v;
   int causal, dtype;

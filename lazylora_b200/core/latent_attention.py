@@ -266,6 +266,8 @@ def _packed(q, k_nope, k_pe, v, cu_q, cu_k, scale, causal):
     if cu_q.dim() != 1 or cu_q.shape[0] < 1:
         raise ValueError("cu_q and cu_k: int32 [sequences + 1]")
     B = cu_q.shape[0] - 1
+    if B == 0 and (Tq or Tk):
+        raise ValueError("cu_q and cu_k: rows without a sequence")
     cu_q, cu_k = _ints(cu_q, torch.int32, B + 1, "cu_q"), _ints(cu_k, torch.int32, B + 1, "cu_k")
     (q, qs), (k_nope, ks), (v, vs) = _view(q), _view(k_nope), _view(v)
     k_pe, ps = (None, _NO_STRIDES) if k_pe is None else _view(k_pe)
@@ -282,7 +284,8 @@ def latent_attention_forward(q: torch.Tensor, k_nope: torch.Tensor, k_pe: Option
 
     q [Tq, H, d_n + d_r], k_nope [Tk, H, d_n], k_pe [Tk, d_r] shared by the heads (None: d_r = 0),
     v [Tk, H, d_v]; sequence b is rows cu_q[b] .. cu_q[b + 1] of the queries and cu_k[b] .. cu_k[b + 1]
-    of the keys (int32; the first is 0 and the last the number of rows). causal: query i of a sequence
+    of the keys (int32; the first is 0 and the last the number of rows, which check_status() holds them to: rows
+    outside every sequence are not written). causal: query i of a sequence
     sees keys j <= i + keys - queries, so its last query sees them all; a query that sees none gets
     zeros and lse = -inf. d_n and d_v 64 or 128, d_r 0 or 64; scale > 0."""
     stream = _stream(q, k_nope, k_pe, v, cu_q, cu_k)

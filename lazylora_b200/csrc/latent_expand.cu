@@ -3,7 +3,8 @@
 //   s_ij = scale q_i . k_j (visible j),  p = softmax(s),  o_i = sum_j p_ij v_j,
 //   dv_j = sum_i p_ij g_i,  dp_ij = g_i . v_j,  ds_ij = p_ij (dp_ij - g_i . o_i) scale,
 //   dq_i = sum_j ds_ij k_j,  dk_j = sum_i ds_ij q_i;  dk_pe sums dk's rotary part over the heads.
-// Tiles are dealt from the cumulative lengths on the device; nothing is read back.
+// Tiles are dealt from the cumulative lengths on the device; nothing is read back. Lengths that do not cover the
+// rows are cut to them, and recorded by a warp without other work in the last block (the lightest tile, or none).
 #include "latent_ops.cuh"
 
 namespace ll {
@@ -25,7 +26,7 @@ namespace ll {
 // Softmax: a thread owns a row. As the row's reference only has to be within 2^8 of its running maximum,
 // O_t is rescaled only when some row of the warp passes that. P is rounded to the 16-bit type (the tensor
 // cores' operand, the output's own precision); sums in fp32 of the unrounded values.
-constexpr int kExThreads = 384;        // warps 0-3, 4-7: softmax of tile 0, 1; 8: TMA; 9: MMA; 10, 11: none
+constexpr int kExThreads = 384;        // warps 0-3, 4-7: softmax of tile 0, 1; 8: TMA; 9: MMA; 10: checks; 11: none
 // Registers: launched with 168 a thread (64,512 a block); the third warpgroup gives some of its up to the two
 // softmax warpgroups: 224 * 256 + 56 * 128 = 176 * 256 + 152 * 128 = 64,512. (The backward's loading and issuing
 // warps spill below 152, 4 % of a packed step; its element-wise warps need no more than 176.)
@@ -277,6 +278,10 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
       volatile int keep = 0;
       mbar_wait_sleep(drain, 0, &keep, a.st, 109, 64);
       __syncwarp();
+    } else if (warp == 10 && blockIdx.x == gridDim.x - 1) {
+      check_cu(a.cu_q, a.B, a.Tq, a.st, 75);
+      check_cu(a.cu_k, a.B, a.Tk, a.st, 76);
+      __syncwarp();
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kExRegsMore));
@@ -407,7 +412,8 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_fwd(const __grid_constant_
 //   dk, dv: S^T 0 (64), dP^T 64 (64), dV 128 (128), dK 256 (192), P^T 448 (32), dS^T 480 (32)
 // Threads: warps 0-3 and 4-7 the element-wise work, each group half of a tile's columns; 8 TMA; 9 the
 // products of S and dP; 11 the sums (a warp that has issued a batch gets on only as the tensor cores take it
-// up, so one issuer alone would leave them idle for its waits); 10 (dk, dv) the queries' statistics.
+// up, so one issuer alone would leave them idle for its waits); 10 (dk, dv) the queries' statistics, (dq) the
+// lengths' check.
 struct ExBwdArgs {
   const int32_t *cu_q, *cu_k;
   const void *g, *o;
@@ -627,6 +633,10 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dq(const __grid_constant__
       if (lead) mma_commit(&drain[1]);
       volatile int keep = 0;
       mbar_wait_sleep(&drain[1], 0, &keep, a.st, 135, 64);
+      __syncwarp();
+    } else if (warp == 10 && blockIdx.x == gridDim.x - 1) {
+      check_cu(a.cu_q, a.B, a.Tq, a.st, 77);
+      check_cu(a.cu_k, a.B, a.Tk, a.st, 78);
       __syncwarp();
     }
   } else {
@@ -902,6 +912,11 @@ __global__ void __launch_bounds__(kExThreads, 1) k_ex_dkv(const __grid_constant_
       __syncwarp();
     } else if (warp == 10) {
       // ------------------------------------------------- statistics of the steps' queries
+      if (a.Tq == 0 && blockIdx.x == gridDim.x - 1) {      // (with queries, k_ex_dq has checked)
+        check_cu(a.cu_q, a.B, 0, a.st, 77);
+        check_cu(a.cu_k, a.B, a.Tk, a.st, 78);
+        __syncwarp();
+      }
       for (int i = 0; i < n; i++) {
         const int s = i % kExQStages;
         mbar_wait_sleep(&q_rel[s], ((i / kExQStages) & 1) ^ 1, abort_flag, a.st, 149, 64);

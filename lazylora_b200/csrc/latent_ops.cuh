@@ -181,6 +181,14 @@ LL_DEV void seq_range(const int32_t* cu, int b, int total, int& lo, int& hi) {
   hi = min(max(cu[b + 1], lo), total);
 }
 
+// Records cumulative lengths that do not start at 0, rise and end at the tensor's rows (a warp).
+LL_DEV void check_cu(const int32_t* cu, int B, int total, DevStatus* st, int where) {
+  for (int b = threadIdx.x & 31; b <= B; b += 32) {
+    const int at = cu[b];
+    if ((b == 0 && at != 0) || (b < B ? cu[b + 1] < at : at != total)) report(st, LL_ERR_RANGE, where, b);
+  }
+}
+
 // The tile-th tile of `rows` rows over all sequences, counted from the first or (FROM_END) from the last
 // one, for a whole warp: true and (b, first row within the sequence) when there is one. Lanes scan 32
 // sequences at a time. The causal kernels count from the side on which a sequence's tiles are longest, so

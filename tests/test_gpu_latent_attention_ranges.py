@@ -47,6 +47,49 @@ def test_paged_lengths_that_fill_the_block_table_are_fine():
 
 
 # ------------------------------------------------------------------------------------------- expanded
+@pytest.mark.parametrize("which", ["cu_q", "cu_k"])
+@pytest.mark.parametrize("cu", [[1, 70, 100], [0, 70, 99], [0, 70, 101], [0, 101, 100], [0, -1, 100], [-5, 70, 100]])
+def test_expanded_reports_cumulative_lengths_that_do_not_cover_the_rows(which, cu):
+    """100 rows in two sequences: cumulative lengths that start past 0, fall, or end elsewhere are recorded
+    by the forward and by the backward."""
+    from lazylora_b200.core import latent_attention as A
+    q, kn, kp, v, cq, ck, go = _expand_case(BF, [70, 30], [70, 30], 2, 128, 64, 128, 1)
+    out, lse = A.latent_attention_forward(q, kn, kp, v, cq, ck, 0.1)
+    A.latent_attention_backward(go, out, lse, q, kn, kp, v, cq, ck, 0.1)
+    A.check_status()
+    bad = torch.tensor(cu, dtype=torch.int32, device="cuda")
+    cq, ck = (bad, ck) if which == "cu_q" else (cq, bad)
+    A.latent_attention_forward(q, kn, kp, v, cq, ck, 0.1)
+    _raises_once()
+    A.latent_attention_backward(go, out, lse, q, kn, kp, v, cq, ck, 0.1)
+    _raises_once()
+
+
+def test_expanded_backward_reports_cumulative_lengths_without_queries():
+    """No query rows at all: the gradients of the keys are zeros, and bad lengths of theirs are recorded too."""
+    from lazylora_b200.core import latent_attention as A
+    q, kn, kp, v, cq, ck, go = _expand_case(BF, [0, 0], [40, 30], 2, 128, 64, 128, 1)
+    lse = torch.zeros(2, 0, device="cuda")
+    d = A.latent_attention_backward(go, go, lse, q, kn, kp, v, cq, ck, 0.1)
+    A.check_status()
+    assert all(bool((t == 0).all()) for t in d[1:])
+    ck[2] = 69
+    A.latent_attention_backward(go, go, lse, q, kn, kp, v, cq, ck, 0.1)
+    _raises_once()
+
+
+def test_expanded_refuses_rows_without_sequences():
+    from lazylora_b200.core import latent_attention as A
+    z = lambda *s: torch.zeros(*s, dtype=BF, device="cuda")  # noqa: E731
+    none = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for tq, tk in ((4, 4), (4, 0), (0, 4)):
+        x = (z(tq, 2, 192), z(tk, 2, 128), z(tk, 64), z(tk, 2, 128), none, none, 0.1)
+        with pytest.raises(ValueError):
+            A.latent_attention_forward(*x)
+        with pytest.raises(ValueError):
+            A.latent_attention_backward(z(tq, 2, 128), z(tq, 2, 128), torch.zeros(2, tq, device="cuda"), *x)
+
+
 def _wide(seed, ql, kl, grow):
     """fp16 operands whose P (dP - delta) passes 65504 while the gradients, which carry the scale and small
     queries and keys, do not: |g| about 4000 and |v| about 32, or |g| about 1500, both growing along the rows
