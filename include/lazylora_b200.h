@@ -370,8 +370,8 @@ const char* ll_profile_launch_name(int i);
  * outside the table, a slot outside the cache, a page outside it, a length that its block table does
  * not hold) are never followed but recorded; a bounded wait that runs out likewise:
  * ll_latent_status(stream) synchronises, returns the first one recorded since the last call on the
- * current device and clears it. A token with a bad position or slot is not written; the attention of a
- * sequence with a bad value is void. */
+ * current device and clears it. A token with a bad position or slot is not written; a bad page's keys
+ * count as rows of zeros; a bad length is cut to what its table or tensor holds. */
 int ll_latent_status(void* stream);
 
 /* New tokens into the paged cache [pages][page_size][d_c + d_r]: token t's row kv[t] (d_c latent

@@ -185,7 +185,8 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
     """(out [B, Tq, H, d_c], lse fp32 [B, Tq, H]) of the absorbed form.
 
     q [B, Tq, H, d_c + d_r]; cache [pages, page_size, d_c + d_r] (page_size a multiple of 8);
-    block_table int32 [B, max_pages]; seq_lens int32 [B], the cached rows of each sequence with the
+    block_table int32 [B, max_pages] (a page outside the cache is recorded for check_status(), its keys count as
+    rows of zeros); seq_lens int32 [B], the cached rows of each sequence with the
     Tq queries' own tokens last (0 to max_pages * page_size; others are recorded for check_status()).
     Query t of sequence b sees its first seq_lens[b] - Tq + t + 1 rows; one that sees none gets zeros and
     lse = -inf. d_c 128, 256, 384 or 512; d_r 0 or 64; scale > 0."""
@@ -323,5 +324,6 @@ def latent_attention_backward(g: torch.Tensor, out: torch.Tensor, lse: torch.Ten
 
 def check_status():
     """Synchronise and raise if a call since the last check met a position, slot, page or length out of range
-    (nothing is read or written outside; a sequence's attention is then void) or a bounded wait that ran out."""
+    (nothing is read or written outside, but the attention of such a sequence is not its formula's) or a
+    bounded wait that ran out."""
     L.check(L.load().ll_latent_status(L.stream_ptr()), "latent attention")

@@ -46,6 +46,18 @@ def test_paged_lengths_that_fill_the_block_table_are_fine():
     _check_paged(out, lse, q, rows, 128, 0.1)
 
 
+@pytest.mark.parametrize("page", [-1, 10 ** 6])
+def test_paged_page_out_of_range_reads_zeros(page):
+    """A page outside the cache is recorded, and its keys are rows of zeros (scores of 0, values of 0)."""
+    from lazylora_b200.core import latent_attention as A
+    q, cache, bt, sl, rows = _paged_case(BF, [30, 90], 1, 4, 128, 64, 8, 4)
+    bt[1, 3] = page
+    rows[1][24:32] = 0
+    out, lse = A.paged_latent_attention(q, cache, bt, sl, 128, 0.1)
+    _raises_once()
+    _check_paged(out, lse, q, rows, 128, 0.1)
+
+
 # ------------------------------------------------------------------------------------------- expanded
 @pytest.mark.parametrize("which", ["cu_q", "cu_k"])
 @pytest.mark.parametrize("cu", [[1, 70, 100], [0, 70, 99], [0, 70, 101], [0, 101, 100], [0, -1, 100], [-5, 70, 100]])
