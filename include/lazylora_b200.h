@@ -436,7 +436,8 @@ int ll_latent_backward(const ll_latent_packed* a, const void* g, int64_t g_strid
                        void* workspace, size_t workspace_bytes, void* stream);
 
 /* One product per head: y[t][h] = x[t][h] . W[h], bf16 with fp32 accumulation; W[h] is [N][K] (w_nk
- * 1, y = x W^T) or [K][N] (0), w_stride_h apart with leading dimension ldw. */
+ * 1, y = x W^T) or [K][N] (0), w_stride_h apart with leading dimension ldw. Its bounded waits are
+ * recorded for ll_gemm_bf16_status. */
 int ll_gemm_bf16_heads(int T, int H, int N, int K, const void* x, int64_t x_stride_t, int64_t x_stride_h,
                        const void* W, int64_t w_stride_h, int64_t ldw, int w_nk, void* y, int64_t y_stride_t,
                        int64_t y_stride_h, void* stream);

@@ -24,6 +24,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib as L
+from . import dense
 
 _DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 
@@ -325,5 +326,9 @@ def latent_attention_backward(g: torch.Tensor, out: torch.Tensor, lse: torch.Ten
 def check_status():
     """Synchronise and raise if a call since the last check met a position, slot, page or length out of range
     (nothing is read or written outside, but the attention of such a sequence is not its formula's) or a
-    bounded wait that ran out."""
-    L.check(L.load().ll_latent_status(L.stream_ptr()), "latent attention")
+    bounded wait that ran out, head_linear's included (they are recorded with those of core.dense, whose
+    check_status() this calls too)."""
+    try:
+        L.check(L.load().ll_latent_status(L.stream_ptr()), "latent attention")
+    finally:
+        dense.check_status()
