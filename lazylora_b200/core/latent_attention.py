@@ -177,7 +177,8 @@ def rotate_positions(x: torch.Tensor, positions: torch.Tensor, table: torch.Tens
 
 
 @functools.lru_cache(maxsize=256)
-def _paged_workspace(B: int, Tq: int, H: int, d_c: int) -> int:
+def _paged_workspace(device: int, B: int, Tq: int, H: int, d_c: int) -> int:
+    """Bytes on the current device, which is `device` (they go by its SMs)."""
     return _lib().ll_paged_latent_workspace_bytes(B, Tq, H, d_c)
 
 
@@ -214,7 +215,7 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
     if B == 0 or Tq == 0 or H == 0:
         return out, lse
     lib, cs = _lib(), cv[1]
-    n = _paged_workspace(B, Tq, H, d_c)
+    n = _paged_workspace(_device(), B, Tq, H, d_c)
     ws = src.new_empty(n, dtype=torch.uint8)
     rc = lib.ll_paged_latent_attention(src.data_ptr(), qs[0], qs[2] if H > 1 else qs[1], cache.data_ptr(), cs[0], cs[1],
                                        pages, page_size, block_table.data_ptr(), block_table.stride(0),

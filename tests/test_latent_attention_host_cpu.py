@@ -39,3 +39,29 @@ def test_check_status_covers_the_per_head_products(monkeypatch, latent, dense):
         A.check_status()
     assert lib.words == {"latent": 0, "dense": 0}, "both are read, whichever raised"
     A.check_status()
+
+
+def test_paged_workspace_is_the_current_devices(monkeypatch):
+    """The size goes by the device's SMs, so one device's is not handed to another."""
+    from lazylora_b200.core import latent_attention as A
+    sizes, given, device = {0: 1000, 1: 5000}, [], [0]
+
+    class Lib:
+        def ll_paged_latent_workspace_bytes(self, *a):
+            return sizes[device[0]]
+
+        def ll_paged_latent_attention(self, *a):
+            given.append((device[0], a[-2]))
+            return 0
+
+    monkeypatch.setattr(A, "_library", Lib())
+    monkeypatch.setattr(A, "_device", lambda: device[0])
+    monkeypatch.setattr(A, "_stream", lambda *tensors: 0)
+    A._paged_workspace.cache_clear()
+    z = lambda *s, dt=torch.bfloat16: torch.zeros(*s, dtype=dt)  # noqa: E731
+    try:
+        for device[0] in (0, 1, 0):
+            A.paged_latent_attention(z(1, 1, 2, 192), z(2, 8, 192), z(1, 1, dt=torch.int32), z(1, dt=torch.int32), 128, 0.1)
+    finally:
+        A._paged_workspace.cache_clear()
+    assert given == [(0, 1000), (1, 5000), (0, 1000)]
