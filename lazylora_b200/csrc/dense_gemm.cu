@@ -276,7 +276,8 @@ __global__ void __launch_bounds__(kDnThreads, 1) k_dense_gemm(const __grid_const
       int j, m0, n0, hd;
       tile_of(u, j, m0, n0, hd);
       const DenseJob& jb = args.job[j];
-      if (!(ok = mbar_wait_sleep(&accfull[ab], abph, abort_flag, st, 48, 512))) break;
+      // (one outcome for the warp, whose lanes load and store together below)
+      if (!(ok = warp_wait_sleep(&accfull[ab], abph, abort_flag, st, 48, 512))) break;
       tc_fence_after();
       const int row = m0 + q * 32 + lane;
       const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + ab * 256;
@@ -558,7 +559,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kDnThreads, 1)
       int j, m0, n0;
       tile_of(u, j, m0, n0);
       const DenseJob& jb = args.job[j];
-      if (!(ok = mbar_wait_sleep(&accfull[ab], abph, abort_flag, st, 58, 512))) break;
+      if (!(ok = warp_wait_sleep(&accfull[ab], abph, abort_flag, st, 58, 512))) break;     // one outcome for the warp
       tc_fence_after();
       const int row = m0 + 128 * (int)rank + q * 32 + lane;
       const uint32_t tbase = tmem + ((uint32_t)(q * 32) << 16) + ab * 256;

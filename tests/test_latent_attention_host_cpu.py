@@ -1,7 +1,10 @@
 """
 The host side of the latent-attention functions without a GPU: what they ask of the library and when, seen
-through a stand-in for it.
+through a stand-in for it; and, in the kernels' source, that no warp can leave a loop apart.
 """
+import os
+import re
+
 import pytest
 import torch
 
@@ -65,3 +68,12 @@ def test_paged_workspace_is_the_current_devices(monkeypatch):
     finally:
         A._paged_workspace.cache_clear()
     assert given == [(0, 1000), (1, 5000), (0, 1000)]
+
+
+def test_epilogue_waits_have_one_outcome_a_warp():
+    """A bounded wait that runs out in some lanes only would let them leave a loop in which the others wait for
+    them (__syncwarp, tcgen05.ld): the dense products' epilogues, whose loops a wait can end, vote on it."""
+    csrc = os.path.join(os.path.dirname(os.path.abspath(_lib.__file__)), "csrc")
+    with open(os.path.join(csrc, "dense_gemm.cu")) as fh:
+        waits = re.findall(r"ok = (\w+)\(&accfull\[ab\], abph", fh.read())
+    assert len(waits) == 2 and set(waits) == {"warp_wait_sleep"}, waits
