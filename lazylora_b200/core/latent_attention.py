@@ -204,8 +204,10 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
     if cv is None or page_size % 8 or cache.numel() == 0:
         raise ValueError("cache: page_size a multiple of 8, contiguous rows, strides multiples of 8, 16-byte aligned")
     if block_table.dim() != 2 or block_table.dtype is not torch.int32 or block_table.shape[0] != B or \
-            block_table.shape[1] == 0 or block_table.stride(1) != 1:
+            block_table.shape[1] == 0:
         raise ValueError("block_table: int32 [B, max_pages]")
+    if block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
     seq_lens = _ints(seq_lens, torch.int32, B, "seq_lens")
     src, qs = _view(q)
     if Tq > 1 and H > 1 and qs[1] != H * qs[2]:                     # the rows (t, h) must be evenly spaced
