@@ -66,7 +66,7 @@ class LatentAttention:
         xb = x.reshape(-1, self.d).to(torch.bfloat16).contiguous()
         N, H = xb.shape[0], self.H
         if N == 0:
-            self._saved = None
+            self._saved = ()
             return torch.empty((0, self.d), dtype=torch.bfloat16, device=x.device)
         q = dense.linear(xb, self.W_q).contiguous().view(N, H, self.d_n + self.d_r)
         A.rotate_positions(q[..., self.d_n:], positions, self.table, interleaved=self.interleaved, out=q[..., self.d_n:])
@@ -83,6 +83,8 @@ class LatentAttention:
         """dL/dx [N, d] bf16 of the last forward."""
         if self._saved is None:
             raise RuntimeError("backward before forward")
+        if not self._saved:                       # a forward without tokens
+            return torch.empty_like(g.reshape(0, self.d), dtype=torch.bfloat16)
         q, k_nope, k_pe, v, out, lse, norm, cu, positions = self._saved
         N, H = q.shape[:2]
         g_out = dense.matmul(g.reshape(N, self.d).to(torch.bfloat16), self.W_o).contiguous().view(N, H, self.d_v)

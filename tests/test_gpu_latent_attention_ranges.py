@@ -7,7 +7,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_latent_attention import BF, HF, U, _check_paged, _expand_case, _paged_case, _within
+from test_gpu_latent_attention import BF, HF, U, _check_paged, _expand_case, _gen, _paged_case, _rand, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -182,3 +182,21 @@ def test_fp16_gradient_of_one_bad_row_stays_in_it():
     got = A.latent_attention_backward(go, out, lse, q, kn, kp, v, cq, ck, 0.07)[0]
     keep = torch.arange(200, device="cuda") != 37
     assert torch.equal(got[keep], want[keep])
+
+
+# ------------------------------------------------------------------------------------------------ layer
+def test_layer_without_tokens():
+    from test_gpu_latent_attention_layer import _layer
+    layer, *_ = _layer(_gen(1), 2, 128, 128, 64, 64, 64, True, False)
+    x = torch.zeros(0, 128, dtype=BF, device="cuda")
+    cu, pos = torch.zeros(1, dtype=torch.int32, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert layer.forward(x, cu, pos).shape == (0, 128)
+    dx = layer.backward(x)
+    assert dx.shape == (0, 128) and dx.dtype is BF
+    # and with tokens again afterwards, and none after those
+    x = _rand(_gen(2), BF, 5, 128)
+    cu, pos = torch.tensor([0, 5], dtype=torch.int32, device="cuda"), torch.arange(5, device="cuda")
+    layer.forward(x, cu, pos)
+    assert layer.backward(x).shape == (5, 128)
+    layer.forward(x[:0], cu[:1], pos[:0])
+    assert layer.backward(x[:0]).shape == (0, 128)
