@@ -13,7 +13,7 @@ heads:
     rest of the layer: the backward returns dL/dx);
   * decode: the absorbed form over a paged cache of (c | k_pe) rows. k_nope's product moves to the
     query, q_nope W_k, and v's to the output, so a token costs d_c + d_r cached values instead of
-    H (d_n + d_r + d_v).
+    H (d_n + d_r + d_v). It takes d_c 128, 256, 384 or 512 (the expanded form is not bound to them).
 
 The projections run on the library's tcgen05 GEMM (core.dense), the rest on core.latent_attention.
 """
@@ -106,6 +106,8 @@ class LatentAttention:
         """y [B, Tq, d] for the last Tq tokens x [B, Tq, d] of B sequences, which are appended to the cache
         [pages, page_size, d_c + d_r] at slots [B Tq] first; seq_lens int32 [B] counts them in."""
         L.require_cuda(x, cache)
+        if self.d_c not in (128, 256, 384, 512):  # (before anything is written to the cache)
+            raise ValueError("decode: d_c 128, 256, 384 or 512")
         B, Tq, _ = x.shape
         N, H = B * Tq, self.H
         xb = x.reshape(N, self.d).to(torch.bfloat16).contiguous()

@@ -200,3 +200,17 @@ def test_layer_without_tokens():
     assert layer.backward(x).shape == (5, 128)
     layer.forward(x[:0], cu[:1], pos[:0])
     assert layer.backward(x[:0]).shape == (0, 128)
+
+
+def test_layer_decode_refuses_other_latents_before_it_writes():
+    """A latent of 192 values trains; decode, whose absorbed form does not take it, leaves the cache alone."""
+    from test_gpu_latent_attention_layer import _layer
+    layer, *_ = _layer(_gen(3), 2, 128, 192, 64, 64, 64, False, False)
+    x = _rand(_gen(4), BF, 5, 128)
+    cu, pos = torch.tensor([0, 5], dtype=torch.int32, device="cuda"), torch.arange(5, device="cuda")
+    assert layer.forward(x, cu, pos).shape == layer.backward(x).shape == (5, 128)
+    cache = torch.full((2, 8, 256), 7.0, dtype=BF, device="cuda")
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        layer.decode(x[:1, None], cache, pos[:1], pos[:1], one[:, None], one)
+    assert bool((cache == 7.0).all())
