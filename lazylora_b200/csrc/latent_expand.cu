@@ -1080,16 +1080,16 @@ static int rows_map(CUtensorMap* m, CUtensorMapDataType dt, const void* base, in
   return make_map_nd(m, dt, base, 3, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
-static int packed_maps(ExTma* tm, const ll_latent_packed* p, uint32_t q_rows = 128, uint32_t k_rows = 128) {
+static int packed_maps(ExTma* tm, const ll_latent_packed* p, uint32_t q_rows = 128) {
   const CUtensorMapDataType dt = p->dtype == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const int dq = p->d_n + p->d_r;
   // an operand without rows is never loaded; its map is any valid one
   if (p->Tq) LL_TRY(rows_map(&tm->q, dt, p->q, p->Tq, p->q_stride_t, p->H, p->q_stride_h, dq, q_rows));
   if (p->Tk) {
-    LL_TRY(rows_map(&tm->kn, dt, p->k_nope, p->Tk, p->k_stride_t, p->H, p->k_stride_h, p->d_n, k_rows));
-    LL_TRY(rows_map(&tm->v, dt, p->v, p->Tk, p->v_stride_t, p->H, p->v_stride_h, p->d_v, k_rows));
+    LL_TRY(rows_map(&tm->kn, dt, p->k_nope, p->Tk, p->k_stride_t, p->H, p->k_stride_h, p->d_n));
+    LL_TRY(rows_map(&tm->v, dt, p->v, p->Tk, p->v_stride_t, p->H, p->v_stride_h, p->d_v));
     if (p->d_r)
-      LL_TRY(make_map_2d(&tm->kp, dt, p->k_pe, 64, (uint64_t)p->Tk, (uint64_t)p->kpe_stride_t * 2, 64, k_rows,
+      LL_TRY(make_map_2d(&tm->kp, dt, p->k_pe, 64, (uint64_t)p->Tk, (uint64_t)p->kpe_stride_t * 2, 64, 128,
                          CU_TENSOR_MAP_SWIZZLE_128B));
     else tm->kp = tm->kn;
   }

@@ -18,9 +18,7 @@ template <>
 struct Num<__nv_bfloat16> {
   static constexpr uint32_t fmt = 1;     // kind::f16 operand format code
   static constexpr bool narrow = false;  // a range short of fp32's
-  static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   LL_DEV static float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-  LL_DEV static __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
   LL_DEV static uint32_t pack(float lo, float hi) {
     const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
@@ -30,9 +28,7 @@ template <>
 struct Num<__half> {
   static constexpr uint32_t fmt = 0;
   static constexpr bool narrow = true;
-  static constexpr CUtensorMapDataType tma = CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   LL_DEV static float to_f(__half v) { return __half2float(v); }
-  LL_DEV static __half from_f(float v) { return __float2half_rn(v); }
   LL_DEV static uint32_t pack(float lo, float hi) {
     const __half2 p = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&p);
