@@ -149,7 +149,7 @@ def expert_bytes(cfg):
 
 
 # --------------------------------------------------------------------- reference arm
-def cpu_reference_sample(cfg, inp_dev, idx, w, n_experts: Optional[int], kind: str = "ref"):
+def cpu_reference_sample(cfg, inp_dev, idx, w, n_experts: Optional[int]):
     """Time the reference CPU path (fwd + bwd sweep) over the layer's active experts, or over a
     seeded sample of n_experts of them with all their routed tokens; returns (seconds, fraction
     of the layer's active experts covered, threads)."""
@@ -157,7 +157,7 @@ def cpu_reference_sample(cfg, inp_dev, idx, w, n_experts: Optional[int], kind: s
     nthreads = os.cpu_count() or 1
     torch.set_num_threads(nthreads)
     os.environ.setdefault("OMP_NUM_THREADS", str(nthreads))
-    kern = O.MXFP4Checker(kind)
+    kern = O.MXFP4Checker("ref")
     active = torch.unique(idx[idx >= 0]).tolist()
     if n_experts is None or n_experts >= len(active):
         pick = active
@@ -215,14 +215,17 @@ def run_reference(args, cfg, rank, world, dist):
     from lazylora_b200.synthetic import make_layer_device
     if rank != 0:
         return
+    from oracle import moe_oracle as O
+    if not os.path.exists(O.REF_SO):       # (the oracle's port of it is not the reference)
+        print(json.dumps({"impl": "reference",
+                          "unavailable": "the reference's C kernel (oracle/_ref) has not been compiled here"}))
+        return
     dev = "cuda" if torch.cuda.is_available() else "cpu"
     if dev == "cpu":
         print(json.dumps({"impl": "reference", "unavailable": "no CUDA device to generate the layer inputs on"}))
         return
     total = replace(cfg, T=cfg.T * world)
     inp = make_layer_device(total, device=dev)
-    from oracle import moe_oracle as O
-    kind = "ref" if os.path.exists(O.REF_SO) else "oracle"
     x_cpu, wr, br = inp["x"].float().cpu(), inp["router_w"].cpu(), inp["router_b"].cpu()
     sample = None if world == 1 else REF_SAMPLE_EXPERTS_EP
     times = []
@@ -232,7 +235,7 @@ def run_reference(args, cfg, rank, world, dist):
         idx, w = O.route(x_cpu, wr, br, total.k)
         t_route = time.perf_counter() - t0
         dt, frac, threads = cpu_reference_sample(total, inp, idx.to(dev), w.to(dev),
-                                                 16 if i < args.warmup else sample, kind)
+                                                 16 if i < args.warmup else sample)
         if i >= args.warmup:
             times.append(t_route + dt / frac)            # seconds for the whole layer
     step_s = statistics.median(times)
@@ -248,7 +251,7 @@ def run_reference(args, cfg, rank, world, dist):
             "scaling": "weak" if world == 1 else "strong", "vs_baseline": None, "dtype": "f32",
             "data": "synthetic", "config": workload_config(cfg, world), "impl": "reference",
             "cpu_baseline": {"value": value, "unit": UNIT, "cores": threads,
-                             "kind": "reference" if kind == "ref" else "port", "sample": desc},
+                             "kind": "reference", "sample": desc},
             "e2e": {"value": value, "unit": UNIT, "h2d_bytes_per_step": 0, "d2h_bytes_per_step": 0}}
     print(json.dumps(line), flush=True)
 
