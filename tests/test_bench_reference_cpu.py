@@ -20,6 +20,6 @@ def test_reference_arm_without_the_reference_is_unavailable(monkeypatch, capsys)
     monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
     monkeypatch.setattr(S, "make_layer_device", never)
     monkeypatch.setattr(bench, "cpu_reference_sample", never)
-    bench.run_reference(SimpleNamespace(steps=20, warmup=5), bench.CONFIGS["c1"], 0, 1, None)
+    bench.run_reference(SimpleNamespace(steps=20, warmup=5), S.CONFIGS["c1"], 0, 1, None)
     line = json.loads(capsys.readouterr().out)
     assert line["impl"] == "reference" and "not been compiled" in line["unavailable"]
