@@ -371,7 +371,10 @@ const char* ll_profile_launch_name(int i);
  * not hold) are never followed but recorded; a bounded wait that runs out likewise:
  * ll_latent_status(stream) synchronises, returns the first one recorded since the last call on the
  * current device and clears it. A token with a bad position or slot is not written; a bad page's keys
- * count as rows of zeros; a bad length is cut to what its table or tensor holds. */
+ * count as rows of zeros; a bad length is cut to what its table or tensor holds. Scores are fp32 and the
+ * weights of a softmax row are held to within 2^8 of its largest: scores (after the scale) may be up to
+ * 2^26 in magnitude. A NaN or infinity in a value row reaches the queries that see it, and may reach others
+ * of the same tile, as 0 times it does in a masked product; never those of another sequence. */
 int ll_latent_status(void* stream);
 
 /* New tokens into the paged cache [pages][page_size][d_c + d_r]: token t's row kv[t] (d_c latent
@@ -429,7 +432,8 @@ int ll_latent_forward(const ll_latent_packed* a, void* out, float* lse, void* st
 
 /* Gradients of the forward for the gradient g of out [Tq][H][d_v] (strides given), from its out and
  * lse: dq [Tq][H][d_n + d_r], dk_nope [Tk][H][d_n], dk_pe [Tk][d_r] (summed over the heads in 32
- * bits, in a fixed order), dv [Tk][H][d_v], contiguous, written whole. Deterministic. */
+ * bits, in a fixed order), dv [Tk][H][d_v], contiguous, written whole. Deterministic. The weights are
+ * computed again from lse: to 2^-22 of the scores' magnitude, as fp32 scores are themselves. */
 size_t ll_latent_backward_workspace_bytes(const ll_latent_packed* a);
 int ll_latent_backward(const ll_latent_packed* a, const void* g, int64_t g_stride_t, int64_t g_stride_h,
                        const void* out, const float* lse, void* dq, void* dk_nope, void* dk_pe, void* dv,

@@ -15,7 +15,9 @@ latent vector per token (d_c values) and one rotary key per token (d_r values, s
 bf16 or fp16 tensors, fp32 softmax statistics and sums; CUDA tensors only, no fallback. Calls run on
 the current stream and synchronise nothing; check_status() raises for what only the device can see (a
 position, slot, page or length out of range). Tensors may be strided: the last dimension contiguous, strides
-multiples of 8 elements and 16-byte aligned starts; others are copied once.
+multiples of 8 elements and 16-byte aligned starts; others are copied once. The functions record nothing
+for autograd: what they return has no graph, also for inputs that require one, and the expanded form's
+gradients are a call of their own.
 """
 import ctypes
 import functools
@@ -191,7 +193,8 @@ def paged_latent_attention(q: torch.Tensor, cache: torch.Tensor, block_table: to
     rows of zeros); seq_lens int32 [B], the cached rows of each sequence with the
     Tq queries' own tokens last (0 to max_pages * page_size; others are recorded for check_status()).
     Query t of sequence b sees its first seq_lens[b] - Tq + t + 1 rows; one that sees none gets zeros and
-    lse = -inf. d_c 128, 256, 384 or 512; d_r 0 or 64; scale > 0."""
+    lse = -inf. d_c 128, 256, 384 or 512; d_r 0 or 64 (append_latent takes 16 and more: without rotary values
+    the rows are the program's own to write); scale > 0."""
     stream = _stream(q, cache, block_table, seq_lens)
     dt = _code(q, cache)
     if q.dim() != 4 or cache.dim() != 3 or q.shape[3] != cache.shape[2]:

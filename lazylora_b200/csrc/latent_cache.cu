@@ -8,11 +8,12 @@
 //
 // Bound by bytes at prompt sizes and by launch latency at a decode step. One block takes a token; an item
 // is 16 contiguous bytes in and out: 8 rotary values (pairs side by side), 8 + 8 of two halves (two such
-// pieces), or 8 latent values to copy. A thread requests its first four items before the token's position
+// pieces), or 8 latent values to copy. A thread requests its first two items before the token's position
 // and its table row (which the heads share through L1) have arrived: three dependent loads become two.
 // Offsets are 64-bit: a cache passes 2^32 bytes.
 // Measured: 9001 tokens with 64 heads (171 MB) 38 us, 4.5 TB/s, 69 % of the copy rate (four items ahead: 56 us, 320
-// threads: 46 us); a decode step of 40 tokens 2.9 us.
+// threads: 46 us); a decode step of 40 tokens 2.9 us. At 64 heads a token has 584 items and a block takes 512
+// at a time, so the last 72 (the latent row) are requested only after the first ones' stores.
 #include "latent_ops.cuh"
 
 namespace ll {

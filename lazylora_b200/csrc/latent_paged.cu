@@ -34,8 +34,10 @@
 // (512 TFLOP/s), one of 700 keys at 32 heads 11 us with the join. In the steady state a tile takes 3700
 // cycles of which its load takes 3500: with 64 query rows in shared memory (74 KB) only two 74 KB tiles fit,
 // so while one is computed (1150 cycles S^T, 850 softmax, 600 O^T) one load is in flight, and it shares the
-// shared-memory ports with the products' operands. Prefetching tiles into L2 and issuing S^T of the next
-// tile ahead both measured slower.
+// shared-memory ports with the products' operands (a 64 x 64 x 16 product reads 4 KB of them, 32 cycles, as
+// long as it takes). The steps are three quarters of the long case (25 tiles an SM, 49 us); the rest is
+// the start, the first maxima, the fp32 pieces written and read again, and the join's launch. Prefetching
+// tiles into L2 and issuing S^T of the next tile ahead both measured slower.
 //
 // Rows of the last tile past the sequence's end, which may hold anything, are set to zero in shared
 // memory before the second product (0 * NaN would reach the sums) and masked by their index.
@@ -336,7 +338,7 @@ __global__ void __launch_bounds__(kPgThreads, 1) k_paged(const __grid_constant__
   } else {
     // ------------------------------------------------- softmax, rescaling and the outputs
     // A wait that ran out does not leave the loops: the other waits then return at once, every
-    // barrier still meets all 128 threads, and the results are void (the status says so).
+    // barrier still meets all 256 threads, and the results are void (the status says so).
     const int quarter = warp % 4, side = warp / 4, key_in = quarter * 16 + lane % 16;
     const int r0 = (side * 2 + lane / 16) * NQ;          // the thread's first query row in the tile
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
@@ -581,7 +583,9 @@ __global__ void __launch_bounds__(128 * GRP) k_paged_combine(const PagedArgs a, 
 }
 
 // Row tiles of a sequence, their height (a multiple of 16, the tiles' rows nearly equal) and the
-// number of ranges the key tiles are dealt into, so that about every SM has one CTA.
+// number of ranges the key tiles are dealt into, so that about every SM has one CTA. The number is a whole
+// one: 51 to 73 row tiles fill 102 to 146 of 148 SMs, but 75 (4801 query rows a sequence) to 100 are not split
+// and fill 75 to 100 (75 tokens of 64 heads against 3000 keys: 97 us).
 struct PagedPlan {
   int RT, NT, G;
   size_t part, ml;        // workspace floats
@@ -611,7 +615,11 @@ static int run_paged(const PagedTma& tm, const PagedArgs& a, int NT, cudaStream_
   else if (NT == 48) LL_TRY((launch_paged<T, 48>(tm, a, smem, s)));
   else LL_TRY((launch_paged<T, 64>(tm, a, smem, s)));
   if (a.G == 1) return LL_OK;
-  if (a.G > 8 * a.B)         // more than about eight pieces a sequence
+  // Four groups a row from about eight pieces a sequence on. Whole calls with four groups and with one, B
+  // sequences of 3000 keys at 64 heads: B = 8 21 and 29 us, 16 30.1 and 30.5, 24 39 and 34.5, 48 69 and 50.
+  // The host knows the mean alone: one sequence of 70 thousand keys among 23 of at most 500 is cut into some
+  // 120 pieces and takes 107 us by this rule, 42 with four groups.
+  if (a.G > 8 * a.B)
     return launch_pdl("k_paged_combine", k_paged_combine<T, 4, 1>, dim3((unsigned)a.B * a.rows), dim3(512), 0, s, a, NT);
   return launch_pdl("k_paged_combine", k_paged_combine<T, 1, 4>, dim3((unsigned)a.B * ((a.rows + 3) / 4)), dim3(128), 0,
                     s, a, NT);

@@ -214,3 +214,47 @@ def test_layer_decode_refuses_other_latents_before_it_writes():
     with pytest.raises(ValueError):
         layer.decode(x[:1, None], cache, pos[:1], pos[:1], one[:, None], one)
     assert bool((cache == 7.0).all())
+
+
+# ------------------------------------------------------------------------------------------ large scores
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_of_large_magnitude(dt, sign):
+    """Scores of 2^25 to 2^26, each one exact product, so far apart that a row's largest ones (2 or 46 equal
+    ones) share its softmax: out is the mean of their values (the shares carry one common factor and are
+    rounded to the type: u, and the output once more), lse their score plus the log of their number (fp32 of
+    that size: 2^-22 relative)."""
+    from lazylora_b200.core import latent_attention as A
+    n, H, scale = 300, 3, 0.5
+    g = _gen(12)
+    steps = 1 + (torch.arange(n, device="cuda") % 150).clamp_max(127) / 128
+    key = (sign * 16384 * steps).to(dt)
+    assert bool((key.double() == sign * 16384 * steps.double()).all())
+    score = key.double() * 4096 * scale
+    top = (score == score.max()).double()
+    top /= top.sum()
+    lse_want = score.max() - torch.log(top.max())
+    # absorbed
+    rows = _rand(g, dt, n, 192)
+    rows[:, 0] = key
+    q = torch.zeros(1, 1, H, 192, dtype=dt, device="cuda")
+    q[..., 0] = 4096
+    pages = (n + 7) // 8
+    cache = torch.zeros(pages, 8, 192, dtype=dt, device="cuda")
+    cache.view(-1, 192)[:n] = rows
+    bt = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    out, lse = A.paged_latent_attention(q, cache, bt, torch.tensor([n], dtype=torch.int32, device="cuda"), 128, scale)
+    want = (top @ rows[:, :128].double()).expand(1, 1, H, 128)
+    _within(out, want, 2 * U[dt] * (top @ rows[:, :128].double().abs()))
+    _within(lse, lse_want.expand(1, 1, H), lse_want.abs() * 2.0 ** -22)
+    # expanded: as many queries as there are row tiles for, not causal
+    k, v = _rand(g, dt, n, H, 128), _rand(g, dt, n, H, 128)
+    k[..., 0] = key[:, None]
+    qe = torch.zeros(260, H, 128, dtype=dt, device="cuda")
+    qe[..., 0] = 4096
+    cq, ck = (torch.tensor([0, m], dtype=torch.int32, device="cuda") for m in (260, n))
+    out, lse = A.latent_attention_forward(qe, k, None, v, cq, ck, scale, causal=False)
+    want = torch.einsum("j,jhd->hd", top, v.double()).expand(260, H, 128)
+    _within(out, want, 2 * U[dt] * torch.einsum("j,jhd->hd", top, v.double().abs()))
+    _within(lse, lse_want.expand(H, 260), lse_want.abs() * 2.0 ** -22)
+    A.check_status()
