@@ -144,6 +144,8 @@ inline int make_act_maps(CUtensorMap* maps, int n, const __half* base, int64_t r
   return LL_OK;
 }
 
+// Lets the kernel be launched with up to `bytes` of dynamic shared memory on the current device. The limit only
+// rises: a smaller launch from another thread must not lower it between this call and its launch.
 int set_smem_attr(const void* func, int bytes);
 
 template <int EPI, int NMAT, int NB, bool COLSCALE, int N_MAX>

@@ -89,7 +89,22 @@ int make_map_2d(CUtensorMap* m, CUtensorMapDataType dt, const void* base, uint64
 }
 
 int set_smem_attr(const void* func, int bytes) {
+  struct Limit {
+    const void* func;
+    int dev, bytes;
+  };
+  static Limit limits[2048];      // some 80 kernels a device
+  static int n = 0;
+  static std::mutex mu;
+  int dev = 0;
+  LL_CUDA(cudaGetDevice(&dev));
+  std::lock_guard<std::mutex> lock(mu);
+  int i = 0;
+  while (i < n && (limits[i].func != func || limits[i].dev != dev)) i++;
+  if (i < n && bytes <= limits[i].bytes) return LL_OK;
   LL_CUDA(cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (i == n && n < (int)(sizeof(limits) / sizeof(limits[0]))) limits[n++] = {func, dev, 0};
+  if (i < n) limits[i].bytes = bytes;
   return LL_OK;
 }
 

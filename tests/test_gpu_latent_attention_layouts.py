@@ -143,3 +143,41 @@ def test_decode_step_in_a_graph():
         assert torch.equal(y, step(caches[1]))
     assert torch.equal(caches[0], caches[1])
     A.check_status()
+
+
+def test_two_host_threads():
+    """Calls of different widths from two threads, whose kernels take different amounts of shared memory."""
+    import threading
+    from lazylora_b200.core import latent_attention as A
+    paged = [_paged_case(BF, [300, 40], 1, 64, d_c, 64, 8, d_c) for d_c in (512, 128)]
+    g = _gen(14)
+    cu = torch.tensor([0, 200], dtype=torch.int32, device="cuda")
+    packed = [(_rand(g, BF, 200, 2, d), _rand(g, BF, 200, 2, 64 if i else 128), None if i else _rand(g, BF, 200, 64),
+               _rand(g, BF, 200, 2, 64), cu, cu, 0.1) for i, d in enumerate((192, 64))]
+    heads = [(_rand(g, BF, 40, 8, 128), _rand(g, BF, 8, 64 + 448 * i, 128)) for i in range(2)]
+
+    def step(i):
+        out = A.paged_latent_attention(*paged[i][:4], (512, 128)[i], 0.1)
+        o, lse = A.latent_attention_forward(*packed[i])
+        return (*out, o, *A.latent_attention_backward(o, o, lse, *packed[i]), A.head_linear(*heads[i]))
+    alone = [step(i) for i in range(2)]
+    torch.cuda.synchronize()
+    faults = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(400):
+                    got = step(i)
+                torch.cuda.current_stream().synchronize()
+                if not all(x is y or torch.equal(x, y) for x, y in zip(got, alone[i])):
+                    faults.append("other results")
+        except Exception as e:  # noqa: BLE001
+            faults.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not faults, faults
+    A.check_status()
